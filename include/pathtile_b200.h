@@ -269,7 +269,8 @@ PT_API int pt_kernel_info(int path, int B, int H, int L, int K, int* out, int n)
  * consumer waited for a tile, bit 1 the producer waited for an in-flight copy
  * to drain, bit 2 the producer waited for consumers to finish a stage; the
  * tensor-core kernels add bit 3 (converter waits), bit 4 (MMA issuer waits) and
- * bit 5 (epilogue waits); bit 6 a peer's dK row never arrived (pt_dx_dk_allreduce).  Reads (and
+ * bit 5 (epilogue waits); bit 6 a peer's dK row never arrived (pt_dx_dk_allreduce);
+ * bits 7 and 8 a state slot past its cache or named twice (pt_scan_step, pt_causal_conv_step).  Reads (and
  * with clear != 0, resets) the word of the current device; synchronises the
  * device.  The reference has no device-side error channel (its kernels return
  * silently on L > 48, kernels/warp_tiled_ampere.py:390).
@@ -338,6 +339,116 @@ PT_API int pt_last_cuda_error(void);
 
 /* Library version: major*10000 + minor*100 + patch. */
 PT_API int pt_version(void);
+
+/* ------------------------------------------------------------------------
+ * Sequence operators: causal convolution, selective scan, fused norm.
+ *
+ * Activations are [batch, len, dim] with contiguous channels and any batch and
+ * step strides (in elements), in fp32, bf16 or fp16 (`dtype`); outputs are
+ * contiguous.  Sums, states and statistics are held in fp32.  `lengths`
+ * (int32 [batch], NULL: all `len`) are the rows' valid steps, clamped to
+ * 0..len: steps behind them are not read, their outputs (and gradients) are 0
+ * and the state passes them unchanged.  No pointer needs more alignment than
+ * its element type; 16-byte aligned rows move in wide words.  There is no
+ * counterpart in the reference.
+ */
+#define PT_F32 0
+#define PT_BF16 1
+#define PT_F16 2
+
+#define PT_CONV_MAX_TAPS 8
+#define PT_SCAN_MAX_STATE 64
+#define PT_NORM_MAX_WIDTH 32768
+
+/* y[b,t,d] = act(bias[d] + sum_{j<taps} w[d,j] x[b,t-taps+1+j,d]), act = silu or
+ * identity; x at the steps -(taps-1)..-1 is the initial state (NULL: 0). */
+typedef struct pt_conv_args {
+  int dtype, param_f32;          /* type of activations; whether w and bias are fp32 (else dtype) */
+  int batch, len, dim, taps;     /* len is 1 for a single-token step */
+  int silu;
+  int cache_rows;                /* step only: rows of `state` */
+  const void* x;
+  long long x_batch, x_step;     /* strides in elements */
+  const void *w, *bias;          /* [dim, taps], [dim] (bias may be NULL) */
+  const void* state_in;          /* [batch, taps-1, dim] contiguous, or NULL */
+  void* state_out;               /* as state_in: the last taps-1 inputs of each row, or NULL.  Step: the cache
+                                    [cache_rows, taps-1, dim], read and shifted in place */
+  long long state_row;           /* step only: elements between the cache's rows */
+  const int *lengths, *slots;    /* slots (step only, may be NULL: row b uses state b): see pt_scan_args */
+  void* y;                       /* [batch, len, dim] */
+  /* backward: dy may have any batch and step strides; the gradients are contiguous and may be NULL */
+  const void* dy;
+  long long dy_batch, dy_step;
+  const void* dstate_out;        /* gradient of state_out, [batch, taps-1, dim] or NULL */
+  void *dx, *dstate_in;
+  void *dw, *dbias;              /* of the parameters' type */
+} pt_conv_args;
+
+PT_API int pt_causal_conv(const pt_conv_args* args, void* stream);
+PT_API size_t pt_causal_conv_bwd_workspace_bytes(const pt_conv_args* args);
+PT_API int pt_causal_conv_bwd(const pt_conv_args* args, void* ws, size_t ws_bytes, void* stream);
+PT_API int pt_causal_conv_step(const pt_conv_args* args, void* stream);
+
+/* Selective (input-dependent) diagonal state space, per batch row and channel d of group g:
+ *   delta = dt + dt_bias (softplus of it if dt_softplus);  h_t[n] = exp(delta A[d,n]) h_{t-1}[n] + delta x B[t,g,n]
+ *   y_t = sum_n C[t,g,n] h_t[n] + D[d] x;  y_t *= silu(z) where z is given. */
+typedef struct pt_scan_args {
+  int dtype;
+  int batch, len, dim, state, groups;  /* dim is a multiple of groups */
+  int dt_softplus;
+  int cache_rows;                      /* step only: rows of `hlast` */
+  const void *x, *dt, *z, *B, *C;      /* z may be NULL; B, C [batch, len, groups, state] */
+  long long x_batch, x_step, dt_batch, dt_step, z_batch, z_step;
+  long long B_batch, B_step, B_group, C_batch, C_step, C_group;
+  const float *A, *D, *dt_bias;        /* [dim, state], [dim] or NULL, [dim] or NULL */
+  const float* h0;                     /* [batch, dim, state] or NULL */
+  float* hlast;                        /* [batch, dim, state] or NULL.  Step: the cache [cache_rows, dim, state],
+                                          updated in place */
+  long long h_row;                     /* step only: elements between the cache's rows */
+  const int* lengths;
+  /* step only, int32 [batch] or NULL (row b uses state b).  A negative slot marks a padding row: its y is 0 and no
+   * state is touched.  So is a row whose slot is past the cache (bit 7, value 128, of the device error word) or
+   * was named by an earlier row (bit 8, value 256). */
+  const int* slots;
+  void* y;
+  float* checkpoints;                  /* pt_scan_checkpoint_bytes bytes: states that the backward pass starts from;
+                                          NULL in a forward pass without a backward one */
+  /* backward; gradients are contiguous and may be NULL */
+  const void* dy;
+  long long dy_batch, dy_step;
+  const float* dhlast;                 /* gradient of hlast or NULL */
+  void *dx, *ddt, *dz, *dB, *dC;
+  float *dA, *dD, *ddt_bias, *dh0;
+} pt_scan_args;
+
+PT_API size_t pt_scan_checkpoint_bytes(const pt_scan_args* args);
+PT_API size_t pt_scan_workspace_bytes(const pt_scan_args* args);
+PT_API int pt_scan(const pt_scan_args* args, void* ws, size_t ws_bytes, void* stream);
+PT_API size_t pt_scan_bwd_workspace_bytes(const pt_scan_args* args);
+PT_API int pt_scan_bwd(const pt_scan_args* args, void* ws, size_t ws_bytes, void* stream);
+PT_API int pt_scan_step(const pt_scan_args* args, void* stream);
+
+/* u = x silu(gate); r = residual + scale u, rounded to the residual's type; y = r / sqrt(mean(r^2) + eps) weight,
+ * the mean over each of `groups` equal parts of a row.  Without gate, scale or residual (NULL) that part falls away. */
+typedef struct pt_norm_args {
+  int dtype, param_f32, residual_f32;  /* residual (and r) in fp32, else dtype */
+  int groups;
+  long long rows;
+  int dim;
+  float eps;
+  const void *x, *gate, *residual;
+  long long x_row, gate_row, residual_row;
+  const void *weight, *scale;
+  void *y, *r;                         /* contiguous; r only (and always) with a residual */
+  /* backward: r is read where there is a residual.  Gradients are contiguous and may be NULL */
+  const void *dy, *dr;                 /* dr: gradient of r, of the residual's type, or NULL */
+  long long dy_row, dr_row;
+  void *dx, *dgate, *dresidual, *dweight, *dscale;
+} pt_norm_args;
+
+PT_API int pt_fused_norm(const pt_norm_args* args, void* stream);
+PT_API size_t pt_fused_norm_bwd_workspace_bytes(const pt_norm_args* args);
+PT_API int pt_fused_norm_bwd(const pt_norm_args* args, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,7 +5,9 @@ K <= 48, behind the operator API of the reference's kernels/warp_tiled.py
 (:mod:`pathtile_b200.warp_tiled`) and kernels/warp_tiled_ampere.py
 (:mod:`pathtile_b200.runtime`).  The math runs in hand-written CUDA kernels in
 ``libpathtile_b200.so`` (C ABI: include/pathtile_b200.h); there is no host
-fallback.
+fallback.  :mod:`pathtile_b200.sequence` adds the operators of a selective
+state space block: causal convolution, selective scan and fused norm, with
+their single-token forms.
 """
 from ._lib import PathTileError
 from .ops import dk, dx, fwd
@@ -18,6 +20,13 @@ from .runtime import (
     depthwise_conv_b200,
     get_runtime,
     install_runtime,
+)
+from .sequence import (
+    causal_conv,
+    causal_conv_step,
+    fused_norm,
+    selective_scan,
+    selective_scan_step,
 )
 from .warp_tiled import DepthwiseConvShared, depthwise_conv_shared
 
@@ -38,4 +47,9 @@ __all__ = [
     "get_runtime",
     "DepthwiseConvShared",
     "depthwise_conv_shared",
+    "causal_conv",
+    "causal_conv_step",
+    "selective_scan",
+    "selective_scan_step",
+    "fused_norm",
 ]

@@ -47,6 +47,13 @@ PT_MAX_K = 48
 PT_MAX_PEERS = 8
 PT_IPC_HANDLE_BYTES = 64
 
+PT_F32 = 0
+PT_BF16 = 1
+PT_F16 = 2
+PT_CONV_MAX_TAPS = 8
+PT_SCAN_MAX_STATE = 64
+PT_NORM_MAX_WIDTH = 32768
+
 
 class LaunchOpts(ctypes.Structure):
     """``pt_launch_opts``: per-call launch options, one entry per path (FWD, DX, DK).
@@ -83,6 +90,57 @@ class PeerGroup(ctypes.Structure):
         ("world", ctypes.c_int),
         ("bufs", ctypes.c_void_p * PT_MAX_PEERS),
         ("epoch", ctypes.c_uint),
+    ]
+
+
+def _fields(kind: object, names: str) -> list[tuple[str, object]]:
+    return [(name, kind) for name in names.split()]
+
+
+class ConvArgs(ctypes.Structure):
+    """``pt_conv_args``."""
+
+    _fields_ = [
+        *_fields(ctypes.c_int, "dtype param_f32 batch len dim taps silu cache_rows"),
+        *_fields(ctypes.c_void_p, "x"),
+        *_fields(ctypes.c_longlong, "x_batch x_step"),
+        *_fields(ctypes.c_void_p, "w bias state_in state_out"),
+        *_fields(ctypes.c_longlong, "state_row"),
+        *_fields(ctypes.c_void_p, "lengths slots y dy"),
+        *_fields(ctypes.c_longlong, "dy_batch dy_step"),
+        *_fields(ctypes.c_void_p, "dstate_out dx dstate_in dw dbias"),
+    ]
+
+
+class ScanArgs(ctypes.Structure):
+    """``pt_scan_args``."""
+
+    _fields_ = [
+        *_fields(ctypes.c_int, "dtype batch len dim state groups dt_softplus cache_rows"),
+        *_fields(ctypes.c_void_p, "x dt z B C"),
+        *_fields(ctypes.c_longlong, "x_batch x_step dt_batch dt_step z_batch z_step"),
+        *_fields(ctypes.c_longlong, "B_batch B_step B_group C_batch C_step C_group"),
+        *_fields(ctypes.c_void_p, "A D dt_bias h0 hlast"),
+        *_fields(ctypes.c_longlong, "h_row"),
+        *_fields(ctypes.c_void_p, "lengths slots y checkpoints dy"),
+        *_fields(ctypes.c_longlong, "dy_batch dy_step"),
+        *_fields(ctypes.c_void_p, "dhlast dx ddt dz dB dC dA dD ddt_bias dh0"),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    """``pt_norm_args``."""
+
+    _fields_ = [
+        *_fields(ctypes.c_int, "dtype param_f32 residual_f32 groups"),
+        *_fields(ctypes.c_longlong, "rows"),
+        *_fields(ctypes.c_int, "dim"),
+        *_fields(ctypes.c_float, "eps"),
+        *_fields(ctypes.c_void_p, "x gate residual"),
+        *_fields(ctypes.c_longlong, "x_row gate_row residual_row"),
+        *_fields(ctypes.c_void_p, "weight scale y r dy dr"),
+        *_fields(ctypes.c_longlong, "dy_row dr_row"),
+        *_fields(ctypes.c_void_p, "dx dgate dresidual dweight dscale"),
     ]
 
 
@@ -131,6 +189,19 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                     _vp]),
     "pt_dx_dk_allreduce_fused": (_c_int, [_c_int, _c_int, _c_int, _c_int]),
     "pt_allreduce_peer": (_c_int, [_fp, _c_int, _c_int, _vp, _vp]),
+    "pt_causal_conv": (_c_int, [_vp, _vp]),
+    "pt_causal_conv_bwd_workspace_bytes": (_c_size, [_vp]),
+    "pt_causal_conv_bwd": (_c_int, [_vp, _vp, _c_size, _vp]),
+    "pt_causal_conv_step": (_c_int, [_vp, _vp]),
+    "pt_scan_checkpoint_bytes": (_c_size, [_vp]),
+    "pt_scan_workspace_bytes": (_c_size, [_vp]),
+    "pt_scan": (_c_int, [_vp, _vp, _c_size, _vp]),
+    "pt_scan_bwd_workspace_bytes": (_c_size, [_vp]),
+    "pt_scan_bwd": (_c_int, [_vp, _vp, _c_size, _vp]),
+    "pt_scan_step": (_c_int, [_vp, _vp]),
+    "pt_fused_norm": (_c_int, [_vp, _vp]),
+    "pt_fused_norm_bwd_workspace_bytes": (_c_size, [_vp]),
+    "pt_fused_norm_bwd": (_c_int, [_vp, _vp, _c_size, _vp]),
 }
 
 _lock = threading.Lock()

@@ -17,6 +17,7 @@
 #include "pt_kernels.cuh"
 #include "pt_peer.cuh"
 #include "pt_registry.h"
+#include "pt_seq.h"
 #include "pt_tc.h"
 
 // Device error word (one per device context); kernels receive its address.
@@ -876,6 +877,19 @@ size_t dk_ws_bytes(const Plan& p) {
 }
 
 }  // namespace
+
+// What the sequence operators' entry points (pt_seq_api.cu) need of this file.
+namespace pt {
+int seq_device(int* sm_count, unsigned** err) {
+  DeviceInfo* di = nullptr;
+  const int rc = current_device(di);
+  if (rc != PT_OK) return rc;
+  *sm_count = di->sm_count;
+  *err = di->err;
+  return PT_OK;
+}
+int seq_cuda_fail(cudaError_t e) { return cuda_fail(e); }
+}  // namespace pt
 
 extern "C" {
 
