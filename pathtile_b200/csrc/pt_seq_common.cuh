@@ -104,14 +104,112 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 1 / (1 + e^-v).  The fast division returns 0 for divisors past 2^126, where
-// the quotient is below 2^-126.
-__device__ __forceinline__ float sigmoidf(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
-__device__ __forceinline__ float siluf(float v) { return __fdividef(v, 1.f + __expf(-v)); }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 1 / (1 + e^-v): the reciprocal of infinity is 0, so large negative v need no care.
+__device__ __forceinline__ float sigmoidf(float v) { return rcp(1.f + ex2(v * -kLog2e)); }
+__device__ __forceinline__ float siluf(float v) { return v * sigmoidf(v); }
 // d silu(v) / dv, with s = sigmoid(v).
-__device__ __forceinline__ float silu_grad(float v, float s) { return s * (1.f + v * (1.f - s)); }
-// log(1 + e^v); past 20 the 1 is below half a step of e^v.
-__device__ __forceinline__ float softplusf(float v) { return v > 20.f ? v : log1pf(__expf(v)); }
+__device__ __forceinline__ float silu_grad(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
+
+// log(1 + e^v).  With e = e^-|v| <= 1 it is max(v, 0) + log(1 + e), and
+// log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the odd series up to s^13
+// leaves s^14 / 15 < 2e-8 of the value, so small results keep their relative
+// precision (log(1 + e) computed as such would not).
+__device__ __forceinline__ float softplusf(float v) {
+  const float e = ex2(-fabsf(v) * kLog2e);
+  const float s = e * rcp(2.f + e), q = s * s;
+  float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  p = fmaf(p, q, 1.f);
+  // A NaN stays one: fmaxf would drop it, e carries it.
+  return fmaf(s + s, p, fmaxf(v, 0.f));
+}
+
+// Two floats in a 64-bit register pair, for the packed fp32 instructions.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float lo2(F2 v) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  return a;
+}
+__device__ __forceinline__ float hi2(F2 v) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  return b;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 ex2x2(F2 x) { return pack2(ex2(lo2(x)), ex2(hi2(x))); }
+
+// Copies of 4, 8 or 16 bytes from global to shared memory that run on while the thread works.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* smem, const void* gmem) {
+  const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(smem));
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(gmem) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(gmem), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// E floats of shared memory (16-byte aligned where E is 4 or more).
+template <int E>
+__device__ __forceinline__ void put_floats(float* dst, const float (&v)[E]) {
+  if constexpr (E % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i)
+      reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) reinterpret_cast<float2*>(dst)[i] = make_float2(v[2 * i], v[2 * i + 1]);
+  }
+}
+template <int E>
+__device__ __forceinline__ void get_floats(const float* src, float (&v)[E]) {
+  if constexpr (E % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {
+      const float4 f = reinterpret_cast<const float4*>(src)[i];
+      v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 f = reinterpret_cast<const float2*>(src)[i];
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  }
+}
 
 // A row's state slot: -1 where there is none to touch.  Every thread of the
 // block calls it.  A slot at or past the cache's end (bit 7 of the device error

@@ -35,53 +35,79 @@
 namespace pt {
 namespace seq {
 
-constexpr int kScanThreads = 128;
-constexpr int kScanWarps = kScanThreads / 32;
-constexpr int kTile = 16;      // steps per tile, and between checkpoints
-constexpr int kHalf = kTile / 2;
+constexpr int kTile = 16;  // steps per tile, and between checkpoints
+constexpr int kSub = 4;    // backward: steps whose states and decays are in registers together
+
+// A block: 4 warps that scan, 4 warps that stage.
+constexpr int kScanners = 128, kStagers = 128, kBlock = kScanners + kStagers;
+constexpr int kScanWarps = kScanners / 32;
 
 template <int S>
 struct ScanShape {
-  static constexpr int kSlices = S;
-  static constexpr int kStates = 4 * S;                      // padded number of states
-  static constexpr int kWarpCh = 2 * (32 / S);               // channels per warp
-  static constexpr int kCh = kScanWarps * kWarpCh;           // channels per block
-  static constexpr int kRowThreads = kScanThreads / kTile;   // threads that stage one step: 8
-  static constexpr int kE = kCh / kRowThreads;               // channels a thread stages
-  static constexpr int kN = kStates / kRowThreads;           // states a thread stages (may be 1)
+  static constexpr int kStates = 4 * S;                     // padded number of states
+  static constexpr int kWarpCh = 2 * (32 / S);              // channels per scanning warp
+  static constexpr int kCh = kScanWarps * kWarpCh;          // channels per block
+  static constexpr int kRowThreads = kStagers / kTile;      // threads that stage one step: 8
+  static constexpr int kE = kCh / kRowThreads;              // neighbouring channels a thread stages: 16, 8, 4, 2
+  static constexpr int kN = kStates / kRowThreads;          // states a thread stages
 };
+
+// The whole block meets; scanners and stagers call it from their own code.
+__device__ __forceinline__ void meet() { asm volatile("barrier.sync 1, %0;" ::"n"(kBlock) : "memory"); }
 
 // Strides, sizes and flags as the kernels use them.
 struct ScanDims {
   int cblocks, segs, seg_len, row_chunks;
-  int wide;  // bit 0 x, 1 dt, 2 z, 3 dy, 4 contiguous outputs: rows may move in wide words
+  int wide;  // bit 0 x, 1 dt, 2 z, 3 dy, 4 outputs: rows may move in wide words
 };
 
-// Where a block works: its group, channels, segment.
+// A scanning thread's place: 2 channels, 4 states.
 template <int S>
-struct ScanPlace {
+struct Scanner {
   using P = ScanShape<S>;
-  int g, c0, nch;  // group, first channel (of all), channels of this block
-  __device__ __forceinline__ ScanPlace(const pt_scan_args& a, int cblocks, int cb) {
-    const int per = a.dim / a.groups;
-    g = cb / cblocks;
-    const int first = (cb % cblocks) * P::kCh;
-    c0 = g * per + first;
-    nch = min(P::kCh, per - first);
+  int lane, warp, slice, cl, s0, c, mine;  // cl: channel pair in the block, c: of all channels, mine: of the pair that exist
+  __device__ __forceinline__ Scanner(int tid, int c0, int nch) {
+    lane = tid & 31, warp = tid >> 5, slice = lane & (S - 1);
+    cl = warp * P::kWarpCh + 2 * (lane / S), s0 = 4 * slice;
+    c = c0 + cl;
+    mine = max(0, min(2, nch - cl));
   }
 };
 
-// Reads one step's states row (B or C) into shared memory.
-template <class T, int S>
-__device__ __forceinline__ void stage_states(const T* row, int n, bool live, float* dst) {
+// A staging thread's place: one step of the tile, kE channels.
+template <int S>
+struct Stager {
   using P = ScanShape<S>;
-  const int k = static_cast<int>(threadIdx.x) & (P::kRowThreads - 1);
-#pragma unroll
-  for (int i = 0; i < P::kN; ++i) {
-    const int j = k + i * P::kRowThreads;
-    dst[j] = live && j < n ? to_f<T>(row[j]) : 0.f;
+  int tr, pr, col, c, n;  // tr: step, pr: place in the row, col: first channel in the block, c: of all, n: channels that exist
+  __device__ __forceinline__ Stager(int tid, int c0, int nch) {
+    tr = tid / P::kRowThreads, pr = tid % P::kRowThreads;
+    col = pr * P::kE;
+    c = c0 + col;
+    n = max(0, min(P::kE, nch - col));
   }
-}
+  __device__ __forceinline__ void params(const float* p, float (&out)[P::kE]) const {
+#pragma unroll
+    for (int i = 0; i < P::kE; ++i) out[i] = p && i < n ? __ldg(p + c + i) : 0.f;
+  }
+};
+
+// One step's B or C row on its way to shared memory.
+template <class T, int S>
+struct StateRow {
+  using P = ScanShape<S>;
+  T v[P::kN];
+  __device__ __forceinline__ void load(const T* row, int n, bool live, int k) {
+#pragma unroll
+    for (int i = 0; i < P::kN; ++i) {
+      const int j = k + i * P::kRowThreads;
+      v[i] = live && j < n ? __ldg(row + j) : from_f<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void store(float* dst, int k) const {
+#pragma unroll
+    for (int i = 0; i < P::kN; ++i) dst[k + i * P::kRowThreads] = to_f<T>(v[i]);
+  }
+};
 
 __device__ __forceinline__ int scan_row_length(const pt_scan_args& a, int b) {
   if (!a.lengths) return a.len;
@@ -89,253 +115,377 @@ __device__ __forceinline__ int scan_row_length(const pt_scan_args& a, int b) {
   return n < 0 ? 0 : n > a.len ? a.len : n;
 }
 
-// This thread's decay rates times log2 e: exp(delta A) = 2^(delta A2).
+// A thread's values of [2 channels][4 states] are two packed pairs per channel.
+using Quad = F2[2][2];
+
+// A state array [dim, state] in global memory (fp32): this thread's values.
 template <int S>
-__device__ __forceinline__ void load_rates(const pt_scan_args& a, int c, int nvalid_c, int s0, float (&A2)[2][4]) {
+__device__ __forceinline__ void load_states(const float* p, const pt_scan_args& a, const Scanner<S>& me, Quad& h) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 2; ++i) {
+    const float* q = p + static_cast<long long>(me.c + i) * a.state + me.s0;
+    if (i < me.mine && (a.state & 3) == 0 && me.s0 < a.state && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      const float4 v = *reinterpret_cast<const float4*>(q);
+      h[i][0] = pack2(v.x, v.y), h[i][1] = pack2(v.z, v.w);
+    } else {
+      float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      A2[i][j] = i < nvalid_c && s0 + j < a.state
-                     ? __ldg(a.A + static_cast<long long>(c + i) * a.state + s0 + j) * kLog2e
-                     : 0.f;
+      for (int j = 0; j < 4; ++j) v[j] = i < me.mine && me.s0 + j < a.state ? q[j] : 0.f;
+      h[i][0] = pack2(v[0], v[1]), h[i][1] = pack2(v[2], v[3]);
+    }
+  }
+}
+template <int S>
+__device__ __forceinline__ void store_states(float* p, const pt_scan_args& a, const Scanner<S>& me, const Quad& h) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float* q = p + static_cast<long long>(me.c + i) * a.state + me.s0;
+    const float v[4] = {lo2(h[i][0]), hi2(h[i][0]), lo2(h[i][1]), hi2(h[i][1])};
+    if (i < me.mine && (a.state & 3) == 0 && me.s0 < a.state && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i < me.mine && me.s0 + j < a.state) q[j] = v[j];
+    }
+  }
 }
 
-// A state array [rows, dim, state] (fp32): this thread's 2 x 4 values.
-__device__ __forceinline__ void load_states(const float* p, const pt_scan_args& a, int c, int nvalid_c, int s0,
-                                            float (&h)[2][4]) {
+// Decay rates times log2 e: exp(delta A) = 2^(delta A2).
+template <int S>
+__device__ __forceinline__ void load_rates(const pt_scan_args& a, const Scanner<S>& me, Quad& A2) {
+  load_states(a.A, a, me, A2);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      h[i][j] = i < nvalid_c && s0 + j < a.state ? p[static_cast<long long>(c + i) * a.state + s0 + j] : 0.f;
-}
-__device__ __forceinline__ void store_states(float* p, const pt_scan_args& a, int c, int nvalid_c, int s0,
-                                             const float (&h)[2][4]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i < nvalid_c && s0 + j < a.state) p[static_cast<long long>(c + i) * a.state + s0 + j] = h[i][j];
+    for (int p = 0; p < 2; ++p) A2[i][p] = mul2(A2[i][p], pack2(kLog2e, kLog2e));
 }
 
-// Sum of v0 (for the pair's first channel) and v1 (second) over a channel's S
-// lanes: an even lane gets the first channel's, an odd one the second's.
+// A channel pair's values of one step, each twice: ready for packed arithmetic over states.
+struct Both {
+  F2 v[2];
+  __device__ __forceinline__ explicit Both(const float* p) {
+    const float2 f = *reinterpret_cast<const float2*>(p);
+    v[0] = pack2(f.x, f.x), v[1] = pack2(f.y, f.y);
+  }
+};
+// Four states' values of one step, in packed pairs.
+struct Four {
+  F2 v[2];
+  __device__ __forceinline__ explicit Four(const float* p) {
+    const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(p);
+    v[0] = f.x, v[1] = f.y;
+  }
+};
+
+// Sums over a channel's S lanes of the values of two steps and two channels
+// (v[step][channel]).  Lane 0 gets step 0 channel 0, lane 1 step 0 channel 1,
+// lanes 2 and 3 step 1; with two lanes each gets its channel's both steps.
 template <int S>
-__device__ __forceinline__ float sum_slices(float v0, float v1, int slice) {
+__device__ __forceinline__ void sum_slices(float (&v)[2][2], int slice, float& first, float& second) {
   const bool odd = slice & 1;
-  float keep = odd ? v1 : v0;
-  const float send = odd ? v0 : v1;
-  keep += __shfl_xor_sync(0xffffffffu, send, 1);
+  if constexpr (S == 2) {
+    first = (odd ? v[0][1] : v[0][0]) + __shfl_xor_sync(0xffffffffu, odd ? v[0][0] : v[0][1], 1);
+    second = (odd ? v[1][1] : v[1][0]) + __shfl_xor_sync(0xffffffffu, odd ? v[1][0] : v[1][1], 1);
+  } else {
+    const bool up = slice & 2;
+    const float a0 = (up ? v[1][0] : v[0][0]) + __shfl_xor_sync(0xffffffffu, up ? v[0][0] : v[1][0], 2);
+    const float a1 = (up ? v[1][1] : v[0][1]) + __shfl_xor_sync(0xffffffffu, up ? v[0][1] : v[1][1], 2);
+    first = (odd ? a1 : a0) + __shfl_xor_sync(0xffffffffu, odd ? a0 : a1, 1);
 #pragma unroll
-  for (int m = 2; m < S; m *= 2) keep += __shfl_xor_sync(0xffffffffu, keep, m);
-  return keep;
+    for (int m = 4; m < S; m *= 2) first += __shfl_xor_sync(0xffffffffu, first, m);
+    second = 0.f;
+  }
 }
+// Writes what sum_slices left, to rows i and i + 1 of dst.
+template <int S>
+__device__ __forceinline__ void put_sums(float (*dst)[ScanShape<S>::kCh], int i, int cl, int slice, float first,
+                                         float second) {
+  if constexpr (S == 2) {
+    dst[i][cl + slice] = first;
+    dst[i + 1][cl + slice] = second;
+  } else {
+    if (slice < 4) dst[i + (slice >> 1)][cl + (slice & 1)] = first;
+  }
+}
+
+// s + h . c over the pair's states that exist.
+__device__ __forceinline__ float dot2(F2 h, F2 c, float s, int first, int states) {
+  // States past the last one are not the operator's: 0 x inf must not reach the sum.
+  if (first < states) s = fmaf(lo2(h), lo2(c), s);
+  if (first + 1 < states) s = fmaf(hi2(h), hi2(c), s);
+  return s;
+}
+
+// Where a block works.
+template <int S>
+struct ScanBlock {
+  int cb, rest, g, c0, nch;  // block of channels, index of the rest of the grid, group, first channel, channels
+  __device__ __forceinline__ ScanBlock(const pt_scan_args& a, int cblocks) {
+    const int nblk = cblocks * a.groups;
+    cb = static_cast<int>(blockIdx.x) % nblk;
+    rest = static_cast<int>(blockIdx.x) / nblk;
+    const int per = a.dim / a.groups, first = (cb % cblocks) * ScanShape<S>::kCh;
+    g = cb / cblocks;
+    c0 = g * per + first;
+    nch = min(ScanShape<S>::kCh, per - first);
+  }
+};
 
 // ---------------------------------------------------------------- segments
 // Forward (REV false): the state that a segment reaches from zero, and the sum
 // of its deltas.  Backward: the gradient a_t dh_t that leaves the segment at
 // its start when none enters at its end.
+template <int S>
+struct SegmentSmem {
+  using P = ScanShape<S>;
+  float d[2][kTile][P::kCh], v[2][kTile][P::kCh];  // delta; delta x or dout silu(z)
+  float B[2][kTile][P::kStates];
+};
+
 template <class T, int S, bool REV>
-__global__ void __launch_bounds__(kScanThreads)
+__global__ void __launch_bounds__(kBlock, 2)
     seq_scan_segment_kernel(pt_scan_args a, ScanDims dm, float* seg_h, float* seg_d) {
   using P = ScanShape<S>;
-  __shared__ float s_delta[kTile][P::kCh], s_in[kTile][P::kCh];
-  __shared__ __align__(16) float s_B[kTile][P::kStates];
-  const int nblk = dm.cblocks * a.groups;
-  const int cb = static_cast<int>(blockIdx.x) % nblk;
-  const int rest = static_cast<int>(blockIdx.x) / nblk;
+  extern __shared__ __align__(16) unsigned char smem[];
+  auto& sm = *reinterpret_cast<SegmentSmem<S>*>(smem);
+  const ScanBlock<S> at(a, dm.cblocks);
   // The last segment (backward: the first) has none to hand its state to.
-  const int seg = rest % (dm.segs - 1) + (REV ? 1 : 0);
-  const int b = rest / (dm.segs - 1);
-  const ScanPlace<S> at(a, dm.cblocks, cb);
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
-  const int slice = lane & (S - 1), cl = warp * P::kWarpCh + 2 * (lane / S), s0 = 4 * slice;
-  const int mine = max(0, min(2, at.nch - cl));
-  float A2[2][4], h[2][4] = {}, dsum[2] = {0.f, 0.f};
-  load_rates<S>(a, at.c0 + cl, mine, s0, A2);
+  const int seg = at.rest % (dm.segs - 1) + (REV ? 1 : 0), b = at.rest / (dm.segs - 1);
   const int len = scan_row_length(a, b);
   const int t0 = seg * dm.seg_len, t1 = min(t0 + dm.seg_len, a.len);
   const int tiles = (t1 - t0 + kTile - 1) / kTile;
-  const int tr = tid / P::kRowThreads, col = (tid % P::kRowThreads) * P::kE;
-  const int ncol = max(0, min(P::kE, at.nch - col));
-  float bias[P::kE];
-#pragma unroll
-  for (int i = 0; i < P::kE; ++i) bias[i] = i < ncol && a.dt_bias ? __ldg(a.dt_bias + at.c0 + col + i) : 0.f;
-  for (int k = 0; k < tiles; ++k) {
-    const int tile = t0 + (REV ? tiles - 1 - k : k) * kTile;
-    const int t = tile + tr;
-    const bool live = t < len && t < t1;
-    Pack<T, P::kE> in, dt, z;
-    if (live) {
-      const long long c = at.c0 + col;
-      dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + c, ncol, dm.wide & 2);
-      if (REV) {
-        in.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + c, ncol, dm.wide & 8);
-        if (a.z) z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + c, ncol, dm.wide & 4);
-      } else {
-        in.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + c, ncol, dm.wide & 1);
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < P::kE; ++i) {
-      float d = 0.f, v = 0.f;
-      if (live && i < ncol) {
-        d = dt.f(i) + bias[i];
-        if (a.dt_softplus) d = softplusf(d);
-        v = in.f(i);
-        if (REV) {
-          if (a.z) v *= siluf(z.f(i));
+  auto tile_of = [&](int k) { return t0 + (REV ? tiles - 1 - k : k) * kTile; };
+  const int tid = static_cast<int>(threadIdx.x);
+  if (tid >= kScanners) {
+    const Stager<S> me(tid - kScanners, at.c0, at.nch);
+    float bias[P::kE];
+    me.params(a.dt_bias, bias);
+    Pack<T, P::kE> dt, in, z;
+    StateRow<T, S> row;
+    auto load = [&](int k) {
+      const int t = tile_of(k) + me.tr;
+      const bool live = t < len && t < t1;
+      if (live) {
+        dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
+        if constexpr (REV) {
+          in.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + me.c, me.n, dm.wide & 8);
+          if (a.z) z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
         } else {
-          v *= d;
+          in.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
         }
       }
-      s_delta[tr][col + i] = d;
-      s_in[tr][col + i] = v;
+      row.load(REV ? static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group
+                   : static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group,
+               a.state, live, me.pr);
+    };
+    auto convert = [&](int k) {
+      const int t = tile_of(k) + me.tr;
+      float d[P::kE] = {}, v[P::kE] = {};
+      if (t < len && t < t1) {
+#pragma unroll
+        for (int i = 0; i < P::kE; ++i) {
+          const float raw = dt.f(i) + bias[i];
+          d[i] = a.dt_softplus ? softplusf(raw) : raw;
+          v[i] = REV ? (a.z ? in.f(i) * siluf(z.f(i)) : in.f(i)) : d[i] * in.f(i);
+        }
+      }
+      put_floats<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
+      put_floats<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
+      row.store(sm.B[k & 1][me.tr], me.pr);
+    };
+    if (tiles > 0) {
+      load(0);
+      convert(0);
+      if (tiles > 1) load(1);
     }
-    const T* row = REV ? static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group
-                       : static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group;
-    stage_states<T, S>(row, a.state, live, s_B[tr]);
-    __syncthreads();
-#pragma unroll 4
+    meet();
+    for (int k = 0; k < tiles; ++k) {
+      if (k + 1 < tiles) convert(k + 1);
+      if (k + 2 < tiles) load(k + 2);
+      meet();
+    }
+    return;
+  }
+  const Scanner<S> me(tid, at.c0, at.nch);
+  Quad A2, h = {};
+  float dsum[2] = {0.f, 0.f};
+  load_rates(a, me, A2);
+  meet();
+  for (int k = 0; k < tiles; ++k) {
+    const int st = k & 1;
+#pragma unroll 8
     for (int q = 0; q < kTile; ++q) {
       const int i = REV ? kTile - 1 - q : q;
-      const float4 Bv = *reinterpret_cast<const float4*>(&s_B[i][s0]);
-      const float Bs[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+      const Both d(&sm.d[st][i][me.cl]), v(&sm.v[st][i][me.cl]);
+      const Four B(&sm.B[st][i][me.s0]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float d = s_delta[i][cl + c], v = s_in[i][cl + c];
-        dsum[c] += d;
+        dsum[c] += lo2(d.v[c]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e = ex2(d * A2[c][j]);
-          h[c][j] = REV ? e * fmaf(v, Bs[j], h[c][j]) : fmaf(e, h[c][j], v * Bs[j]);
+        for (int p = 0; p < 2; ++p) {
+          const F2 e = ex2x2(mul2(d.v[c], A2[c][p]));
+          h[c][p] = REV ? mul2(e, fma2(v.v[c], B.v[p], h[c][p])) : fma2(e, h[c][p], mul2(v.v[c], B.v[p]));
         }
       }
     }
+    meet();
   }
-  const long long row = static_cast<long long>(b) * dm.segs + seg;
-  store_states(seg_h + row * a.dim * a.state, a, at.c0 + cl, mine, s0, h);
-  if (slice == 0)
+  const long long out = static_cast<long long>(b) * dm.segs + seg;
+  store_states(seg_h + out * a.dim * a.state, a, me, h);
+  if (me.slice == 0)
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      if (c < mine) seg_d[row * a.dim + at.c0 + cl + c] = dsum[c];
+      if (c < me.mine) seg_d[out * a.dim + me.c + c] = dsum[c];
 }
 
 // h <- exp(A sum delta of segment s) h + its own state.
+template <int S>
 __device__ __forceinline__ void join_segment(const pt_scan_args& a, const ScanDims& dm, const float* seg_h,
-                                             const float* seg_d, int b, int s, int c, int mine, int s0,
-                                             const float (&A2)[2][4], float (&h)[2][4]) {
+                                             const float* seg_d, int b, int s, const Scanner<S>& me, const Quad& A2,
+                                             Quad& h) {
   const long long row = static_cast<long long>(b) * dm.segs + s;
-  float l[2][4];
-  load_states(seg_h + row * a.dim * a.state, a, c, mine, s0, l);
+  Quad l;
+  load_states(seg_h + row * a.dim * a.state, a, me, l);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float d = i < mine ? seg_d[row * a.dim + c + i] : 0.f;
+    const float d = i < me.mine ? seg_d[row * a.dim + me.c + i] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[i][j] = fmaf(ex2(d * A2[i][j]), h[i][j], l[i][j]);
+    for (int p = 0; p < 2; ++p) h[i][p] = fma2(ex2x2(mul2(pack2(d, d), A2[i][p])), h[i][p], l[i][p]);
   }
 }
 
 // ---------------------------------------------------------------- forward
+template <int S>
+struct ForwardSmem {
+  using P = ScanShape<S>;
+  float d[2][kTile][P::kCh], v[2][kTile][P::kCh], y[2][kTile][P::kCh];  // delta, delta x, sums over states of h C
+  float B[2][kTile][P::kStates], C[2][kTile][P::kStates];
+};
+
 template <class T, int S, bool PAD>
-__global__ void __launch_bounds__(kScanThreads)
+__global__ void __launch_bounds__(kBlock, 2)
     seq_scan_fwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d) {
   using P = ScanShape<S>;
-  __shared__ float s_delta[kTile][P::kCh], s_in[kTile][P::kCh], s_y[kTile][P::kCh];
-  __shared__ __align__(16) float s_B[kTile][P::kStates], s_C[kTile][P::kStates];
-  const int nblk = dm.cblocks * a.groups;
-  const int cb = static_cast<int>(blockIdx.x) % nblk;
-  const int rest = static_cast<int>(blockIdx.x) / nblk;
-  const int seg = rest % dm.segs, b = rest / dm.segs;
-  const ScanPlace<S> at(a, dm.cblocks, cb);
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
-  const int slice = lane & (S - 1), cl = warp * P::kWarpCh + 2 * (lane / S), s0 = 4 * slice;
-  const int mine = max(0, min(2, at.nch - cl));
-  float A2[2][4], h[2][4] = {};
-  load_rates<S>(a, at.c0 + cl, mine, s0, A2);
-  if (a.h0) load_states(a.h0 + static_cast<long long>(b) * a.dim * a.state, a, at.c0 + cl, mine, s0, h);
-  for (int s = 0; s < seg; ++s) join_segment(a, dm, seg_h, seg_d, b, s, at.c0 + cl, mine, s0, A2, h);
+  extern __shared__ __align__(16) unsigned char smem[];
+  auto& sm = *reinterpret_cast<ForwardSmem<S>*>(smem);
+  const ScanBlock<S> at(a, dm.cblocks);
+  const int seg = at.rest % dm.segs, b = at.rest / dm.segs;
   const int len = scan_row_length(a, b);
   const int t0 = seg * dm.seg_len, t1 = min(t0 + dm.seg_len, a.len);
-  const int tr = tid / P::kRowThreads, col = (tid % P::kRowThreads) * P::kE;
-  const int ncol = max(0, min(P::kE, at.nch - col));
-  float bias[P::kE], Dv[P::kE];
-#pragma unroll
-  for (int i = 0; i < P::kE; ++i) {
-    bias[i] = i < ncol && a.dt_bias ? __ldg(a.dt_bias + at.c0 + col + i) : 0.f;
-    Dv[i] = i < ncol && a.D ? __ldg(a.D + at.c0 + col + i) : 0.f;
-  }
-  const long long ckpt_row = (static_cast<long long>(a.len) + kTile - 1) / kTile;
-  for (int tile = t0; tile < t1; tile += kTile) {
-    const int t = tile + tr;
-    const bool live = t < len && t < t1;
-    const long long c = at.c0 + col;
-    Pack<T, P::kE> x, dt, z;
-    if (live) {
-      dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + c, ncol, dm.wide & 2);
-      x.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + c, ncol, dm.wide & 1);
-      if (a.z) z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + c, ncol, dm.wide & 4);
-    }
-    if (a.checkpoints)
-      store_states(a.checkpoints + (b * ckpt_row + tile / kTile) * a.dim * a.state, a, at.c0 + cl, mine, s0, h);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < P::kE; ++i) {
-      float d = 0.f, v = 0.f;
-      if (live && i < ncol) {
-        d = dt.f(i) + bias[i];
-        if (a.dt_softplus) d = softplusf(d);
-        v = d * x.f(i);
+  const int tiles = max(0, (t1 - t0 + kTile - 1) / kTile);
+  const int tid = static_cast<int>(threadIdx.x);
+  if (tid >= kScanners) {
+    const Stager<S> me(tid - kScanners, at.c0, at.nch);
+    float bias[P::kE], Dv[P::kE];
+    me.params(a.dt_bias, bias);
+    me.params(a.D, Dv);
+    // x and z of three tiles: the one whose outputs are next, the one being scanned, the next one.
+    Pack<T, P::kE> dt, x[3], z[3];
+    StateRow<T, S> rowB, rowC;
+    auto load = [&](int k) {
+      const int t = t0 + k * kTile + me.tr;
+      const bool live = t < len && t < t1;
+      if (live) {
+        dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
+        x[2].load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
+        if (a.z) z[2].load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
       }
-      s_delta[tr][col + i] = d;
-      s_in[tr][col + i] = v;
-    }
-    stage_states<T, S>(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live,
-                       s_B[tr]);
-    stage_states<T, S>(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live,
-                       s_C[tr]);
-    __syncthreads();
-#pragma unroll 4
-    for (int i = 0; i < kTile; ++i) {
-      const float4 Bv = *reinterpret_cast<const float4*>(&s_B[i][s0]);
-      const float4 Cv = *reinterpret_cast<const float4*>(&s_C[i][s0]);
-      const float Bs[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, Cs[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
-      float y[2];
+      rowB.load(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live, me.pr);
+      rowC.load(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live, me.pr);
+    };
+    auto convert = [&](int k) {
+      const int t = t0 + k * kTile + me.tr;
+      x[0] = x[1], z[0] = z[1], x[1] = x[2], z[1] = z[2];
+      float d[P::kE] = {}, v[P::kE] = {};
+      if (t < len && t < t1) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float d = s_delta[i][cl + c], v = s_in[i][cl + c];
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          h[c][j] = fmaf(ex2(d * A2[c][j]), h[c][j], v * Bs[j]);
-          // States past the last one are not the operator's: 0 x inf must not reach y.
-          s = PAD && s0 + j >= a.state ? s : fmaf(h[c][j], Cs[j], s);
+        for (int i = 0; i < P::kE; ++i) {
+          const float raw = dt.f(i) + bias[i];
+          d[i] = a.dt_softplus ? softplusf(raw) : raw;
+          v[i] = d[i] * x[1].f(i);
         }
-        y[c] = s;
       }
-      const float sum = sum_slices<S>(y[0], y[1], slice);
-      if (slice < 2) s_y[i][cl + slice] = sum;
-    }
-    __syncthreads();
-    if (t < t1 && ncol > 0) {
+      put_floats<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
+      put_floats<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
+      rowB.store(sm.B[k & 1][me.tr], me.pr);
+      rowC.store(sm.C[k & 1][me.tr], me.pr);
+    };
+    auto finish = [&](int k, const Pack<T, P::kE>& xk, const Pack<T, P::kE>& zk) {
+      const int t = t0 + k * kTile + me.tr;
+      if (t >= t1) return;
       Pack<T, P::kE> out;
+      out.zero();
+      if (t < len) {
+        float y[P::kE];
+        get_floats<P::kE>(&sm.y[k & 1][me.tr][me.col], y);
 #pragma unroll
-      for (int i = 0; i < P::kE; ++i) {
-        float v = 0.f;
-        if (live) {
-          v = s_y[tr][col + i];
-          if (a.D) v = fmaf(Dv[i], x.f(i), v);
-          if (a.z) v *= siluf(z.f(i));
+        for (int i = 0; i < P::kE; ++i) {
+          if (a.D) y[i] = fmaf(Dv[i], xk.f(i), y[i]);
+          if (a.z) y[i] *= siluf(zk.f(i));
+          out.set(i, y[i]);
         }
-        out.set(i, v);
       }
-      out.store(static_cast<T*>(a.y) + (static_cast<long long>(b) * a.len + t) * a.dim + c, ncol, dm.wide & 16);
+      out.store(static_cast<T*>(a.y) + (static_cast<long long>(b) * a.len + t) * a.dim + me.c, me.n, dm.wide & 16);
+    };
+    if (tiles > 0) {
+      load(0);
+      convert(0);
+      if (tiles > 1) load(1);
     }
+    meet();
+    for (int k = 0; k < tiles; ++k) {
+      if (k > 0) finish(k - 1, x[0], z[0]);
+      if (k + 1 < tiles) {
+        convert(k + 1);
+        if (k + 2 < tiles) load(k + 2);
+      } else {
+        x[0] = x[1], z[0] = z[1];
+      }
+      meet();
+    }
+    if (tiles > 0) finish(tiles - 1, x[0], z[0]);
+    return;
+  }
+  const Scanner<S> me(tid, at.c0, at.nch);
+  Quad A2, h = {};
+  load_rates(a, me, A2);
+  if (a.h0) load_states(a.h0 + static_cast<long long>(b) * a.dim * a.state, a, me, h);
+  for (int s = 0; s < seg; ++s) join_segment(a, dm, seg_h, seg_d, b, s, me, A2, h);
+  const long long ckpt_row = (static_cast<long long>(a.len) + kTile - 1) / kTile;
+  meet();
+  for (int k = 0; k < tiles; ++k) {
+    const int st = k & 1;
+    if (a.checkpoints)
+      store_states(a.checkpoints + (b * ckpt_row + t0 / kTile + k) * a.dim * a.state, a, me, h);
+#pragma unroll 4
+    for (int i = 0; i < kTile; i += 2) {
+      float y[2][2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const Both d(&sm.d[st][i + q][me.cl]), v(&sm.v[st][i + q][me.cl]);
+        const Four B(&sm.B[st][i + q][me.s0]), C(&sm.C[st][i + q][me.s0]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+            h[c][p] = fma2(ex2x2(mul2(d.v[c], A2[c][p])), h[c][p], mul2(v.v[c], B.v[p]));
+          if constexpr (PAD) {
+            y[q][c] = dot2(h[c][1], C.v[1], dot2(h[c][0], C.v[0], 0.f, me.s0, a.state), me.s0 + 2, a.state);
+          } else {
+            const F2 s = fma2(h[c][1], C.v[1], mul2(h[c][0], C.v[0]));
+            y[q][c] = lo2(s) + hi2(s);
+          }
+        }
+      }
+      float first, second;
+      sum_slices<S>(y, me.slice, first, second);
+      put_sums<S>(sm.y[st], i, me.cl, me.slice, first, second);
+    }
+    meet();
   }
   if (a.hlast && seg == dm.segs - 1)
-    store_states(a.hlast + static_cast<long long>(b) * a.dim * a.state, a, at.c0 + cl, mine, s0, h);
+    store_states(a.hlast + static_cast<long long>(b) * a.dim * a.state, a, me, h);
 }
 
 // ---------------------------------------------------------------- backward
@@ -374,215 +524,318 @@ __device__ __forceinline__ void sum_channels(float (&v)[8], int lane, float* dst
   }
 }
 
+template <int S>
+struct BackwardSmem {
+  using P = ScanShape<S>;
+  float d[2][kTile][P::kCh];                          // delta
+  float v[2][kTile][P::kCh], w[2][kTile][P::kCh];     // delta x, dout silu(z); then the sums over states of dh B, h C
+  float gA[2][kTile][P::kCh];                         // sums over states of (d log a) A2
+  float B[2][kTile][P::kStates], C[2][kTile][P::kStates];
+  float red[2][kScanWarps][kTile][2 * P::kStates];    // the warps' sums over channels, of dB and dC
+  float4 ck[2][kScanners];                            // the next tile's checkpoint; each thread's own
+  float4 start[kTile / kSub - 1][2][kScanners];       // states at the later parts of the tile
+  float4 accA[2][kScanners];                          // dA
+  float accD[kTile][P::kCh], accb[kTile][P::kCh];     // dD and ddt_bias at the end
+};
+
 template <class T, int S, bool PAD>
-__global__ void __launch_bounds__(kScanThreads)
+__global__ void __launch_bounds__(kBlock, 2)
     seq_scan_bwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d, float* part_bc,
                         float* part_a, float* part_d) {
   using P = ScanShape<S>;
-  extern __shared__ __align__(16) float smem[];
-  float(*s_delta)[P::kCh] = reinterpret_cast<float(*)[P::kCh]>(smem);
-  float(*s_in)[P::kCh] = s_delta + kTile;   // delta x
-  float(*s_dy)[P::kCh] = s_in + kTile;      // dout silu(z)
-  float(*s_gB)[P::kCh] = s_dy + kTile;      // sum over states of dh B
-  float(*s_gA)[P::kCh] = s_gB + kTile;      // sum over states of (d log a) A2
-  float(*s_y)[P::kCh] = s_gA + kTile;       // sum over states of h C
-  float(*s_accD)[P::kCh] = s_y + kTile;     // each staging thread's own sums of dD and ddt_bias
-  float(*s_accb)[P::kCh] = s_accD + kTile;
-  float(*s_B)[P::kStates] = reinterpret_cast<float(*)[P::kStates]>(s_accb + kTile);
-  float(*s_C)[P::kStates] = s_B + kTile;
-  float(*s_red)[kTile][2 * P::kStates] = reinterpret_cast<float(*)[kTile][2 * P::kStates]>(s_C + kTile);  // [warp]
-  const int nblk = dm.cblocks * a.groups;
-  const int cb = static_cast<int>(blockIdx.x) % nblk;
-  const int rest = static_cast<int>(blockIdx.x) / nblk;
-  const int seg = rest % dm.segs, chunk = rest / dm.segs;
-  const ScanPlace<S> at(a, dm.cblocks, cb);
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
-  const int slice = lane & (S - 1), cl = warp * P::kWarpCh + 2 * (lane / S), s0 = 4 * slice;
-  const int mine = max(0, min(2, at.nch - cl));
-  float A2[2][4], dA[2][4] = {};
-  load_rates<S>(a, at.c0 + cl, mine, s0, A2);
-  const int tr = tid / P::kRowThreads, col = (tid % P::kRowThreads) * P::kE;
-  const int ncol = max(0, min(P::kE, at.nch - col));
-#pragma unroll
-  for (int i = 0; i < P::kE; ++i) s_accD[tr][col + i] = s_accb[tr][col + i] = 0.f;
+  extern __shared__ __align__(16) unsigned char smem[];
+  auto& sm = *reinterpret_cast<BackwardSmem<S>*>(smem);
+  const ScanBlock<S> at(a, dm.cblocks);
+  const int seg = at.rest % dm.segs, chunk = at.rest / dm.segs;
   const int t0 = seg * dm.seg_len, t1 = min(t0 + dm.seg_len, a.len);
   const int tiles = max(0, (t1 - t0 + kTile - 1) / kTile);
   const long long ckpt_row = (static_cast<long long>(a.len) + kTile - 1) / kTile;
   const long long all = static_cast<long long>(a.dim) * a.state;
-  for (int b = chunk; b < a.batch; b += dm.row_chunks) {
-    const int len = scan_row_length(a, b);
-    float g[2][4] = {};  // a_{t+1} dh_{t+1}
-    if (a.dhlast) load_states(a.dhlast + b * all, a, at.c0 + cl, mine, s0, g);
-    for (int s = dm.segs - 1; s > seg; --s) join_segment(a, dm, seg_h, seg_d, b, s, at.c0 + cl, mine, s0, A2, g);
-    for (int k = tiles - 1; k >= 0; --k) {
-      const int tile = t0 + k * kTile;
-      const int t = tile + tr;
-      const bool live = t < len && t < t1;
-      const long long c = at.c0 + col;
-      Pack<T, P::kE> x, dt, z, dy;
-      x.zero(), dt.zero(), z.zero(), dy.zero();
-      if (live) {
-        dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + c, ncol, dm.wide & 2);
-        x.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + c, ncol, dm.wide & 1);
-        dy.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + c, ncol, dm.wide & 8);
-        if (a.z) z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + c, ncol, dm.wide & 4);
-      }
-      float h[2][4];
-      load_states(a.checkpoints + (b * ckpt_row + tile / kTile) * all, a, at.c0 + cl, mine, s0, h);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < P::kE; ++i) {
-        float d = 0.f, v = 0.f, w = 0.f;
-        if (live && i < ncol) {
-          d = dt.f(i) + (a.dt_bias ? __ldg(a.dt_bias + c + i) : 0.f);
-          if (a.dt_softplus) d = softplusf(d);
-          v = d * x.f(i);
-          w = dy.f(i);
-          if (a.z) w *= siluf(z.f(i));
-        }
-        s_delta[tr][col + i] = d;
-        s_in[tr][col + i] = v;
-        s_dy[tr][col + i] = w;
-      }
-      stage_states<T, S>(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live,
-                         s_B[tr]);
-      stage_states<T, S>(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live,
-                         s_C[tr]);
-      __syncthreads();
-      // The state in the middle of the tile, then the later half, then the earlier one.
-      float mid[2][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mid[i][j] = h[i][j];
-#pragma unroll 2
-      for (int i = 0; i < kHalf; ++i) {
-        const float4 Bv = *reinterpret_cast<const float4*>(&s_B[i][s0]);
-        const float Bs[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          const float d = s_delta[i][cl + cc], v = s_in[i][cl + cc];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mid[cc][j] = fmaf(ex2(d * A2[cc][j]), mid[cc][j], v * Bs[j]);
-        }
-      }
-#pragma unroll 1
-      for (int half = 1; half >= 0; --half) {
-        const int i0 = half * kHalf;
-        float hs[kHalf + 1][2][4], as[kHalf][2][4];  // hs[i]: the state before step i0 + i
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) hs[0][cc][j] = half ? mid[cc][j] : h[cc][j];
-#pragma unroll
-        for (int i = 0; i < kHalf; ++i) {
-          const float4 Bv = *reinterpret_cast<const float4*>(&s_B[i0 + i][s0]);
-          const float Bs[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const float d = s_delta[i0 + i][cl + cc], v = s_in[i0 + i][cl + cc];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              as[i][cc][j] = ex2(d * A2[cc][j]);
-              hs[i + 1][cc][j] = fmaf(as[i][cc][j], hs[i][cc][j], v * Bs[j]);
-            }
-          }
-        }
-#pragma unroll
-        for (int i = kHalf - 1; i >= 0; --i) {
-          const float4 Bv = *reinterpret_cast<const float4*>(&s_B[i0 + i][s0]);
-          const float4 Cv = *reinterpret_cast<const float4*>(&s_C[i0 + i][s0]);
-          const float Bs[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, Cs[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
-          float bc[8] = {};
-          float gB[2] = {}, gA[2] = {}, yy[2] = {};
-#pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const float d = s_delta[i0 + i][cl + cc], v = s_in[i0 + i][cl + cc], w = s_dy[i0 + i][cl + cc];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool real = !PAD || s0 + j < a.state;
-              const float dh = fmaf(w, Cs[j], g[cc][j]);
-              bc[j] = fmaf(dh, v, bc[j]);
-              bc[4 + j] = fmaf(w, hs[i + 1][cc][j], bc[4 + j]);
-              gB[cc] = real ? fmaf(dh, Bs[j], gB[cc]) : gB[cc];
-              yy[cc] = real ? fmaf(hs[i + 1][cc][j], Cs[j], yy[cc]) : yy[cc];
-              g[cc][j] = as[i][cc][j] * dh;
-              const float dlog = g[cc][j] * hs[i][cc][j];
-              gA[cc] = real ? fmaf(dlog, A2[cc][j], gA[cc]) : gA[cc];
-              dA[cc][j] = fmaf(dlog, d, dA[cc][j]);
-            }
-          }
-          sum_channels<S>(bc, lane, s_red[warp][i0 + i]);
-          const float r0 = sum_slices<S>(gB[0], gB[1], slice);
-          const float r1 = sum_slices<S>(gA[0], gA[1], slice);
-          const float r2 = sum_slices<S>(yy[0], yy[1], slice);
-          if (slice < 2) {
-            s_gB[i0 + i][cl + slice] = r0;
-            s_gA[i0 + i][cl + slice] = r1;
-            s_y[i0 + i][cl + slice] = r2;
-          }
-        }
-      }
-      __syncthreads();
-      if (t < t1 && ncol > 0) {
-        Pack<T, P::kE> ox, odt, oz;
-#pragma unroll
-        for (int i = 0; i < P::kE; ++i) {
-          float gx = 0.f, gd = 0.f, gz = 0.f;
-          if (live && i < ncol) {
-            const float xv = x.f(i), Dv = a.D ? __ldg(a.D + c + i) : 0.f, w = s_dy[tr][col + i];
-            const float raw = dt.f(i) + (a.dt_bias ? __ldg(a.dt_bias + c + i) : 0.f);
-            gx = s_gB[tr][col + i] * s_delta[tr][col + i];
-            if (a.D) gx = fmaf(Dv, w, gx);
-            gd = fmaf(s_gB[tr][col + i], xv, s_gA[tr][col + i] * kLn2);
-            if (a.dt_softplus && raw <= 20.f) gd *= sigmoidf(raw);
-            if (a.z) {
-              const float zv = z.f(i);
-              const float yv = a.D ? fmaf(Dv, xv, s_y[tr][col + i]) : s_y[tr][col + i];
-              gz = dy.f(i) * yv * silu_grad(zv, sigmoidf(zv));
-            }
-            s_accD[tr][col + i] = fmaf(w, xv, s_accD[tr][col + i]);
-            s_accb[tr][col + i] += gd;
-          }
-          ox.set(i, gx), odt.set(i, gd), oz.set(i, gz);
-        }
-        const long long o = (static_cast<long long>(b) * a.len + t) * a.dim + c;
-        if (a.dx) ox.store(static_cast<T*>(a.dx) + o, ncol, dm.wide & 16);
-        if (a.ddt) odt.store(static_cast<T*>(a.ddt) + o, ncol, dm.wide & 16);
-        if (a.dz) oz.store(static_cast<T*>(a.dz) + o, ncol, dm.wide & 16);
-      }
-      if (part_bc) {
-        // [block of the group's channels][batch][len][group][2 * states]
-        const int steps = min(kTile, t1 - tile);
-        for (int i = tid; i < steps * 2 * P::kStates; i += kScanThreads) {
-          const int q = i / (2 * P::kStates), k2 = i % (2 * P::kStates);
-          float s = 0.f;
-#pragma unroll
-          for (int w = 0; w < kScanWarps; ++w) s += s_red[w][q][k2];
-          part_bc[(((static_cast<long long>(cb % dm.cblocks) * a.batch + b) * a.len + tile + q) * a.groups + at.g) *
-                      (2 * P::kStates) +
-                  k2] = s;
-        }
-      }
-    }
-    if (a.dh0 && seg == 0) store_states(a.dh0 + b * all, a, at.c0 + cl, mine, s0, g);
-  }
   const long long piece = static_cast<long long>(chunk) * dm.segs + seg;
-  if (part_a) store_states(part_a + piece * all, a, at.c0 + cl, mine, s0, dA);
-  __syncthreads();
-  for (int i = tid; i < at.nch; i += kScanThreads) {
-    float sD = 0.f, sb = 0.f;
-#pragma unroll
-    for (int q = 0; q < kTile; ++q) sD += s_accD[q][i], sb += s_accb[q][i];
-    part_d[piece * 2 * a.dim + at.c0 + i] = sD;
-    part_d[piece * 2 * a.dim + a.dim + at.c0 + i] = sb;
-  }
-}
+  const int tid = static_cast<int>(threadIdx.x);
+  // Tiles are taken from the last to the first; k counts them in that order.
+  auto tile_of = [&](int k) { return t0 + (tiles - 1 - k) * kTile; };
 
-template <int S>
-constexpr int scan_bwd_smem() {
-  using P = ScanShape<S>;
-  return 4 * (8 * kTile * P::kCh + 2 * kTile * P::kStates + kScanWarps * kTile * 2 * P::kStates);
+  if (tid >= kScanners) {
+    const Stager<S> me(tid - kScanners, at.c0, at.nch);
+    float accD[P::kE] = {}, accb[P::kE] = {};
+    for (int b = chunk; b < a.batch; b += dm.row_chunks) {
+      const int len = scan_row_length(a, b);
+      struct Raw {
+        Pack<T, P::kE> dt, x, z, dy;
+      } next, last;  // of the tile to convert, of the tile whose gradients are to be written
+      StateRow<T, S> rowB, rowC;
+      auto load = [&](int k, Raw& r) {
+        const int t = tile_of(k) + me.tr;
+        if (t < len && t < t1) {
+          r.dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
+          r.x.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
+          r.dy.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + me.c, me.n, dm.wide & 8);
+          if (a.z) r.z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
+        }
+      };
+      auto load_next = [&](int k) {
+        load(k, next);
+        const int t = tile_of(k) + me.tr;
+        const bool live = t < len && t < t1;
+        rowB.load(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live, me.pr);
+        rowC.load(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live, me.pr);
+      };
+      auto convert = [&](int k) {
+        const int t = tile_of(k) + me.tr;
+        float d[P::kE] = {}, v[P::kE] = {}, w[P::kE] = {};
+        if (t < len && t < t1) {
+#pragma unroll
+          for (int i = 0; i < P::kE; ++i) {
+            const float raw = next.dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f);
+            d[i] = a.dt_softplus ? softplusf(raw) : raw;
+            v[i] = d[i] * next.x.f(i);
+            w[i] = a.z ? next.dy.f(i) * siluf(next.z.f(i)) : next.dy.f(i);
+          }
+        }
+        put_floats<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
+        put_floats<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
+        put_floats<P::kE>(&sm.w[k & 1][me.tr][me.col], w);
+        rowB.store(sm.B[k & 1][me.tr], me.pr);
+        rowC.store(sm.C[k & 1][me.tr], me.pr);
+      };
+      auto finish = [&](int k) {
+        const int tile = tile_of(k), t = tile + me.tr, st = k & 1;
+        if (t < t1) {
+          Pack<T, P::kE> ox, odt, oz;
+          ox.zero(), odt.zero(), oz.zero();
+          if (t < len) {
+            float d[P::kE], gB[P::kE], gA[P::kE], y[P::kE];
+            get_floats<P::kE>(&sm.d[st][me.tr][me.col], d);
+            get_floats<P::kE>(&sm.v[st][me.tr][me.col], gB);
+            get_floats<P::kE>(&sm.gA[st][me.tr][me.col], gA);
+            get_floats<P::kE>(&sm.w[st][me.tr][me.col], y);
+#pragma unroll
+            for (int i = 0; i < P::kE; ++i) {
+              const float x = last.x.f(i), dy = last.dy.f(i);
+              const float Dv = a.D && i < me.n ? __ldg(a.D + me.c + i) : 0.f;
+              float w = dy;
+              if (a.z) {
+                const float z = last.z.f(i), s = sigmoidf(z);
+                w *= z * s;
+                oz.set(i, dy * (a.D ? fmaf(Dv, x, y[i]) : y[i]) * silu_grad(z, s));
+              }
+              float gd = fmaf(gB[i], x, gA[i] * kLn2);
+              if (a.dt_softplus)
+                gd *= sigmoidf(last.dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f));
+              ox.set(i, a.D ? fmaf(Dv, w, gB[i] * d[i]) : gB[i] * d[i]);
+              odt.set(i, gd);
+              accD[i] = fmaf(w, x, accD[i]);
+              accb[i] += gd;
+            }
+          }
+          const long long o = (static_cast<long long>(b) * a.len + t) * a.dim + me.c;
+          const bool wide = dm.wide & 16;
+          if (a.dx) ox.store(static_cast<T*>(a.dx) + o, me.n, wide);
+          if (a.ddt) odt.store(static_cast<T*>(a.ddt) + o, me.n, wide);
+          if (a.dz) oz.store(static_cast<T*>(a.dz) + o, me.n, wide);
+        }
+        if (part_bc) {
+          // [block of the group's channels][batch][len][group][2 * states]
+          const int n = min(kTile, t1 - tile) * 2 * P::kStates;
+          const long long row = (static_cast<long long>(at.cb % dm.cblocks) * a.batch + b) * a.len + tile;
+#pragma unroll 4
+          for (int i = tid - kScanners; i < kTile * 2 * P::kStates; i += kStagers) {
+            if (i >= n) break;
+            const int q = i / (2 * P::kStates), k2 = i % (2 * P::kStates);
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < kScanWarps; ++w) s += sm.red[st][w][q][k2];
+            part_bc[((row + q) * a.groups + at.g) * (2 * P::kStates) + k2] = s;
+          }
+        }
+      };
+      if (tiles > 0) {
+        load_next(0);
+        convert(0);
+        if (tiles > 1) load_next(1);
+        load(0, last);
+      }
+      meet();
+      for (int k = 0; k < tiles; ++k) {
+        if (k > 0) {
+          finish(k - 1);
+          load(k, last);
+        }
+        if (k + 1 < tiles) {
+          convert(k + 1);
+          if (k + 2 < tiles) load_next(k + 2);
+        }
+        meet();
+      }
+      if (tiles > 0) finish(tiles - 1);
+      meet();
+    }
+    put_floats<P::kE>(&sm.accD[me.tr][me.col], accD);
+    put_floats<P::kE>(&sm.accb[me.tr][me.col], accb);
+    meet();
+    for (int c = tid - kScanners; c < at.nch; c += kStagers) {
+      float sD = 0.f, sb = 0.f;
+#pragma unroll
+      for (int q = 0; q < kTile; ++q) sD += sm.accD[q][c], sb += sm.accb[q][c];
+      part_d[piece * 2 * a.dim + at.c0 + c] = sD;
+      part_d[piece * 2 * a.dim + a.dim + at.c0 + c] = sb;
+    }
+    return;
+  }
+
+  const Scanner<S> me(tid, at.c0, at.nch);
+  Quad A2;
+  load_rates(a, me, A2);
+  sm.accA[0][tid] = sm.accA[1][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool quads = (a.state & 3) == 0 && (reinterpret_cast<uintptr_t>(a.checkpoints) & 15) == 0;
+  for (int b = chunk; b < a.batch; b += dm.row_chunks) {
+    auto fetch = [&](int k) {
+      const float* ck = a.checkpoints + (b * ckpt_row + tile_of(k) / kTile) * all;
+      if (quads) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i < me.mine && me.s0 < a.state)
+            copy_async<16>(&sm.ck[i][tid], ck + static_cast<long long>(me.c + i) * a.state + me.s0);
+          else
+            sm.ck[i][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      } else {
+        Quad h;
+        load_states(ck, a, me, h);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          sm.ck[i][tid] = make_float4(lo2(h[i][0]), hi2(h[i][0]), lo2(h[i][1]), hi2(h[i][1]));
+      }
+      copy_commit();
+    };
+    if (tiles > 0) fetch(0);
+    Quad g = {};  // a_{t+1} dh_{t+1}
+    if (a.dhlast) load_states(a.dhlast + b * all, a, me, g);
+    for (int s = dm.segs - 1; s > seg; --s) join_segment(a, dm, seg_h, seg_d, b, s, me, A2, g);
+    meet();
+    for (int k = 0; k < tiles; ++k) {
+      const int st = k & 1;
+      Quad first, h;  // the state at the tile's start, and walking on from it
+      copy_wait<0>();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.ck[c][tid]);
+        first[c][0] = h[c][0] = v.x, first[c][1] = h[c][1] = v.y;
+      }
+      if (k + 1 < tiles) fetch(k + 1);
+      // The states at the later parts' starts.
+#pragma unroll 1
+      for (int sub = 0; sub < kTile / kSub - 1; ++sub) {
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) {
+          const int t = sub * kSub + i;
+          const Both d(&sm.d[st][t][me.cl]), v(&sm.v[st][t][me.cl]);
+          const Four B(&sm.B[st][t][me.s0]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              h[c][p] = fma2(ex2x2(mul2(d.v[c], A2[c][p])), h[c][p], mul2(v.v[c], B.v[p]));
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          *reinterpret_cast<ulonglong2*>(&sm.start[sub][c][tid]) = make_ulonglong2(h[c][0], h[c][1]);
+      }
+      Quad dA = {};
+#pragma unroll 1
+      for (int sub = kTile / kSub - 1; sub >= 0; --sub) {
+        const int i0 = sub * kSub;
+        F2 hs[kSub + 1][2][2], as[kSub][2][2];  // hs[i]: the state before step i0 + i
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (sub > 0) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.start[sub - 1][c][tid]);
+            hs[0][c][0] = v.x, hs[0][c][1] = v.y;
+          } else {
+            hs[0][c][0] = first[c][0], hs[0][c][1] = first[c][1];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) {
+          const Both d(&sm.d[st][i0 + i][me.cl]), v(&sm.v[st][i0 + i][me.cl]);
+          const Four B(&sm.B[st][i0 + i][me.s0]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              as[i][c][p] = ex2x2(mul2(d.v[c], A2[c][p]));
+              hs[i + 1][c][p] = fma2(as[i][c][p], hs[i][c][p], mul2(v.v[c], B.v[p]));
+            }
+        }
+        float gB[2][2], gA[2][2], yy[2][2];
+#pragma unroll
+        for (int i = kSub - 1; i >= 0; --i) {
+          const Both d(&sm.d[st][i0 + i][me.cl]), v(&sm.v[st][i0 + i][me.cl]), w(&sm.w[st][i0 + i][me.cl]);
+          const Four B(&sm.B[st][i0 + i][me.s0]), C(&sm.C[st][i0 + i][me.s0]);
+          F2 bB[2], bC[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            F2 sB = 0, sA = 0, sy = 0;  // two zeros each
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              const F2 dh = fma2(w.v[c], C.v[p], g[c][p]);
+              bB[p] = c ? fma2(dh, v.v[c], bB[p]) : mul2(dh, v.v[c]);
+              bC[p] = c ? fma2(w.v[c], hs[i + 1][c][p], bC[p]) : mul2(w.v[c], hs[i + 1][c][p]);
+              g[c][p] = mul2(as[i][c][p], dh);
+              const F2 dlog = mul2(g[c][p], hs[i][c][p]);
+              dA[c][p] = fma2(dlog, d.v[c], dA[c][p]);
+              if constexpr (PAD) {
+                const int f = me.s0 + 2 * p;
+                sB = pack2(dot2(dh, B.v[p], lo2(sB), f, a.state), 0.f);
+                sA = pack2(dot2(dlog, A2[c][p], lo2(sA), f, a.state), 0.f);
+                sy = pack2(dot2(hs[i + 1][c][p], C.v[p], lo2(sy), f, a.state), 0.f);
+              } else {
+                sB = p ? fma2(dh, B.v[p], sB) : mul2(dh, B.v[p]);
+                sA = p ? fma2(dlog, A2[c][p], sA) : mul2(dlog, A2[c][p]);
+                sy = p ? fma2(hs[i + 1][c][p], C.v[p], sy) : mul2(hs[i + 1][c][p], C.v[p]);
+              }
+            }
+            gB[i & 1][c] = lo2(sB) + hi2(sB);
+            gA[i & 1][c] = lo2(sA) + hi2(sA);
+            yy[i & 1][c] = lo2(sy) + hi2(sy);
+          }
+          float bc[8] = {lo2(bB[0]), hi2(bB[0]), lo2(bB[1]), hi2(bB[1]), lo2(bC[0]), hi2(bC[0]), lo2(bC[1]), hi2(bC[1])};
+          sum_channels<S>(bc, me.lane, sm.red[st][me.warp][i0 + i]);
+          if ((i & 1) == 0) {
+            float f0, f1, f2, s0, s1, s2;
+            sum_slices<S>(gB, me.slice, f0, s0);
+            sum_slices<S>(gA, me.slice, f1, s1);
+            sum_slices<S>(yy, me.slice, f2, s2);
+            __syncwarp();  // v and w of these steps have been read by the channel's other lanes
+            put_sums<S>(sm.v[st], i0 + i, me.cl, me.slice, f0, s0);
+            put_sums<S>(sm.gA[st], i0 + i, me.cl, me.slice, f1, s1);
+            put_sums<S>(sm.w[st], i0 + i, me.cl, me.slice, f2, s2);
+          }
+        }
+      }
+      // Tile by tile, so that a long row's sum is not one chain of additions.
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float4 s = sm.accA[c][tid];
+        s.x += lo2(dA[c][0]), s.y += hi2(dA[c][0]), s.z += lo2(dA[c][1]), s.w += hi2(dA[c][1]);
+        sm.accA[c][tid] = s;
+      }
+      meet();
+    }
+    if (a.dh0 && seg == 0) store_states(a.dh0 + b * all, a, me, g);
+    meet();  // the next row's tiles overwrite what this row's last gradients are made from
+  }
+  if (part_a) {
+    Quad dA;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float4 s = sm.accA[c][tid];
+      dA[c][0] = pack2(s.x, s.y), dA[c][1] = pack2(s.z, s.w);
+    }
+    store_states(part_a + piece * all, a, me, dA);
+  }
+  meet();
 }
 
 // dB and dC from the blocks' partial sums, in block order.
@@ -602,14 +855,16 @@ __global__ void seq_scan_bc_kernel(const float* part, int cblocks, long long row
 }
 
 // ---------------------------------------------------------------- one token
+constexpr int kStepThreads = 128;
+
 // A lane holds four states of a channel, S lanes the channel.
 template <class T, int S>
-__global__ void __launch_bounds__(kScanThreads) seq_scan_step_kernel(pt_scan_args a, int cblocks, bool wide,
+__global__ void __launch_bounds__(kStepThreads) seq_scan_step_kernel(pt_scan_args a, int cblocks, bool wide,
                                                                      unsigned* err) {
-  constexpr int kCh = kScanThreads / S;
+  constexpr int kCh = kStepThreads / S;
   const int cb = static_cast<int>(blockIdx.x) % cblocks, b = static_cast<int>(blockIdx.x) / cblocks;
   const int tid = static_cast<int>(threadIdx.x);
-  const int slot = a.slots ? slot_of(a.slots, b, a.cache_rows, err, tid, kScanThreads) : b;
+  const int slot = a.slots ? slot_of(a.slots, b, a.cache_rows, err, tid, kStepThreads) : b;
   const int slice = tid & (S - 1), s0 = 4 * slice;
   const int c = cb * kCh + tid / S;
   const bool in = c < a.dim;
@@ -679,7 +934,7 @@ ScanDims scan_dims(const pt_scan_args& a, const ScanPlan& p) {
   d.wide |= ok(a.dt, a.dt_batch, a.dt_step) ? 2 : 0;
   d.wide |= ok(a.z, a.z_batch, a.z_step) ? 4 : 0;
   d.wide |= ok(a.dy, a.dy_batch, a.dy_step) ? 8 : 0;
-  d.wide |= rows && aligned(a.y, word) && aligned(a.dx, word) && aligned(a.ddt, word) && aligned(a.dz, word) ? 16 : 0;
+  d.wide |= ok(a.y, 0, 0) && ok(a.dx, 0, 0) && ok(a.ddt, 0, 0) && ok(a.dz, 0, 0) ? 16 : 0;
   return d;
 }
 
@@ -688,6 +943,18 @@ inline size_t segment_floats(const pt_scan_args& a, const ScanPlan& p) {
   if (p.segs <= 1) return 0;
   const size_t n = static_cast<size_t>(a.batch) * p.segs * a.dim * (static_cast<size_t>(a.state) + 1);
   return (n + 3) / 4 * 4;
+}
+
+// Launches a kernel whose shared memory is one Smem.
+template <class Smem, class K, class... A>
+cudaError_t launch_with(K kernel, long long grid, int threads, cudaStream_t stream, A... args) {
+  constexpr int bytes = static_cast<int>(sizeof(Smem));
+  if (bytes > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+  }
+  kernel<<<static_cast<unsigned>(grid), threads, bytes, stream>>>(args...);
+  return cudaGetLastError();
 }
 
 template <class T>
@@ -700,17 +967,12 @@ cudaError_t scan_fwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
     const long long blocks = static_cast<long long>(p.cblocks) * a.groups * a.batch;
     if (blocks * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     if (p.segs > 1) {
-      seq_scan_segment_kernel<T, S, false>
-          <<<static_cast<unsigned>(blocks * (p.segs - 1)), kScanThreads, 0, stream>>>(a, dm, seg_h, seg_d);
-      const cudaError_t e = cudaGetLastError();
+      const cudaError_t e = launch_with<SegmentSmem<S>>(
+          seq_scan_segment_kernel<T, S, false>, blocks * (p.segs - 1), kBlock, stream, a, dm, seg_h, seg_d);
       if (e != cudaSuccess) return e;
     }
-    const unsigned grid = static_cast<unsigned>(blocks * p.segs);
-    if (a.state == 4 * S)
-      seq_scan_fwd_kernel<T, S, false><<<grid, kScanThreads, 0, stream>>>(a, dm, seg_h, seg_d);
-    else
-      seq_scan_fwd_kernel<T, S, true><<<grid, kScanThreads, 0, stream>>>(a, dm, seg_h, seg_d);
-    return cudaGetLastError();
+    auto kernel = a.state == 4 * S ? seq_scan_fwd_kernel<T, S, false> : seq_scan_fwd_kernel<T, S, true>;
+    return launch_with<ForwardSmem<S>>(kernel, blocks * p.segs, kBlock, stream, a, dm, seg_h, seg_d);
   });
 }
 
@@ -731,18 +993,14 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
     if (blocks * a.batch * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     cudaError_t e;
     if (p.segs > 1) {
-      seq_scan_segment_kernel<T, S, true>
-          <<<static_cast<unsigned>(blocks * a.batch * (p.segs - 1)), kScanThreads, 0, stream>>>(a, dm, seg_h, seg_d);
-      if ((e = cudaGetLastError()) != cudaSuccess) return e;
+      e = launch_with<SegmentSmem<S>>(seq_scan_segment_kernel<T, S, true>, blocks * a.batch * (p.segs - 1),
+                                               kBlock, stream, a, dm, seg_h, seg_d);
+      if (e != cudaSuccess) return e;
     }
     auto kernel = a.state == 4 * S ? seq_scan_bwd_kernel<T, S, false> : seq_scan_bwd_kernel<T, S, true>;
-    constexpr int smem = scan_bwd_smem<S>();
-    if (smem > 48 * 1024 &&
-        (e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess)
-      return e;
-    kernel<<<static_cast<unsigned>(blocks * pieces), kScanThreads, smem, stream>>>(
-        a, dm, seg_h, seg_d, a.dB || a.dC ? part_bc : nullptr, a.dA ? part_a : nullptr, part_d);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = launch_with<BackwardSmem<S>>(kernel, blocks * pieces, kBlock, stream, a, dm, seg_h, seg_d,
+                                        a.dB || a.dC ? part_bc : nullptr, a.dA ? part_a : nullptr, part_d);
+    if (e != cudaSuccess) return e;
     if (a.dB || a.dC) {
       const long long n = rows * 8 * S;
       if (n > 0) {
@@ -765,11 +1023,11 @@ template <class T>
 cudaError_t scan_step(const pt_scan_args& a, int slices, unsigned* err, cudaStream_t stream) {
   return by_slices(slices, [&](auto sc) -> cudaError_t {
     constexpr int S = decltype(sc)::value;
-    const int cblocks = static_cast<int>(cdiv(a.dim, kScanThreads / S));
+    const int cblocks = static_cast<int>(cdiv(a.dim, kStepThreads / S));
     const long long grid = static_cast<long long>(cblocks) * a.batch;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     const bool wide = a.state % 4 == 0 && a.h_row % 4 == 0 && aligned(a.hlast, 16) && aligned(a.A, 16);
-    seq_scan_step_kernel<T, S><<<static_cast<unsigned>(grid), kScanThreads, 0, stream>>>(a, cblocks, wide, err);
+    seq_scan_step_kernel<T, S><<<static_cast<unsigned>(grid), kStepThreads, 0, stream>>>(a, cblocks, wide, err);
     return cudaGetLastError();
   });
 }
