@@ -23,7 +23,8 @@ cudaError_t launch_reduce(const float* part, int chunks, long long stride, long 
 
 // How the convolution's backward pass is cut (pt_seq_conv.cuh).
 struct ConvBwdPlan {
-  int v, cblocks, tblocks, steps, chunks;
+  int v, tx, cblocks, chunks;
+  long long per;
 };
 
 // How a scan is cut: `segs` pieces of `seg_len` steps run side by side.

@@ -10,7 +10,7 @@ namespace seq {
 
 // Defined and instantiated per activation type in pt_seq_conv_*.cu and pt_seq_scan_*.cu.
 template <class T>
-cudaError_t conv_fwd(const pt_conv_args&, cudaStream_t);
+cudaError_t conv_fwd(const pt_conv_args&, int, cudaStream_t);
 template <class T>
 cudaError_t conv_bwd(const pt_conv_args&, float*, int, cudaStream_t);
 template <class T>
@@ -118,7 +118,7 @@ int pt_causal_conv(const pt_conv_args* a, void* stream) {
   int sms;
   unsigned* err;
   PT_TRY(seq_device(&sms, &err));
-  return status(by_type(a->dtype, [&](auto t) { return conv_fwd<decltype(t)>(*a, static_cast<cudaStream_t>(stream)); }));
+  return status(by_type(a->dtype, [&](auto t) { return conv_fwd<decltype(t)>(*a, sms, static_cast<cudaStream_t>(stream)); }));
 }
 
 size_t pt_causal_conv_bwd_workspace_bytes(const pt_conv_args* a) {

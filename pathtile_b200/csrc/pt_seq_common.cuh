@@ -141,14 +141,10 @@ __device__ __forceinline__ F2 pack2(float a, float b) {
   return r;
 }
 __device__ __forceinline__ float lo2(F2 v) {
-  float a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  return a;
+  return __uint_as_float(static_cast<unsigned>(v));
 }
 __device__ __forceinline__ float hi2(F2 v) {
-  float a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  return b;
+  return __uint_as_float(static_cast<unsigned>(v >> 32));
 }
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   F2 r;

@@ -1,13 +1,16 @@
 // pt_seq_conv.cuh -- causal depthwise convolution of a few taps (1..8) over
 // [batch, len, dim]: forward, backward and the single-token step.
 //
-// A thread owns V neighbouring channels of one batch row and walks TS steps;
-// the last K-1 inputs and the taps stay in registers, so every input is read
-// once from memory (plus K-1 steps of overlap per thread) and the kernel is
-// bound by the two (backward: three) streams it moves.  V is the widest word
-// (up to 16 bytes forward, 8 backward) that every pointer, stride and row
-// length allows; loads of U steps are issued together so that enough bytes are
-// in flight.  Channels are the fast axis of the block, steps the slow one.
+// A thread owns V neighbouring channels and walks a stretch of steps; the last
+// K inputs and the taps stay in registers, so every input is read once from
+// memory (plus K-1 steps of overlap per stretch).  All rows' steps are laid end
+// to end and cut into equal stretches, so that every thread has the same work
+// whatever the batch; a stretch that crosses into the next row starts anew
+// there.  V is the widest word (up to 16 bytes forward, 8 backward) that every
+// pointer, stride and row length allows.  The loads of the next U steps are
+// under way while U steps are computed, in packed fp32 arithmetic.  The taps
+// come through shared memory: read straight, a warp's taps lie V x K floats
+// apart and cost more than the steps.
 //
 // Backward, walking forward in time: g[t] = dy[t] act'(pre[t]) with pre
 // recomputed from the window, dx[t-K+1] = sum_j w[j] g[t-j] from the window of
@@ -22,13 +25,34 @@ namespace pt {
 namespace seq {
 
 constexpr int kConvThreads = 128;
-constexpr int kConvBwdTx = 32, kConvBwdTy = kConvThreads / kConvBwdTx;
+constexpr int kConvAhead = 4;  // steps whose loads are under way together
 
 __device__ __forceinline__ int row_length(const int* lengths, int b, int len) {
   if (!lengths) return len;
   const int n = __ldg(lengths + b);
   return n < 0 ? 0 : n > len ? len : n;
 }
+
+// V channels' values in packed pairs (V = 1: the second half is idle).
+template <int V>
+struct Packed {
+  static constexpr int N = (V + 1) / 2;
+  F2 p[N];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = 0;
+  }
+  template <class T>
+  __device__ __forceinline__ void from(const Pack<T, V>& a) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = pack2(a.f(2 * i), 2 * i + 1 < V ? a.f(2 * i + 1 < V ? 2 * i + 1 : 0) : 0.f);
+  }
+  template <class T>
+  __device__ __forceinline__ void to(Pack<T, V>& a) const {
+#pragma unroll
+    for (int v = 0; v < V; ++v) a.set(v, v & 1 ? hi2(p[v / 2]) : lo2(p[v / 2]));
+  }
+};
 
 template <class T, int K, int V>
 struct ConvRow {
@@ -50,176 +74,246 @@ struct ConvRow {
     }
   }
 };
-
 template <class T, int K, int V>
-__device__ __forceinline__ void conv_params(const pt_conv_args& a, int c, float (&w)[K][V], float (&bias)[V]) {
+__device__ __forceinline__ ConvRow<T, K, V> conv_row(const pt_conv_args& a, int b, int c) {
+  return ConvRow<T, K, V>{
+      static_cast<const T*>(a.x) + b * a.x_batch + c,
+      a.state_in ? static_cast<const T*>(a.state_in) + static_cast<long long>(b) * (K - 1) * a.dim + c : nullptr,
+      a.x_step, a.dim, row_length(a.lengths, b, a.len)};
+}
+
+// Taps and bias of V channels.
+template <int K, int V>
+struct Taps {
+  Packed<V> w[K], bias;
+  __device__ __forceinline__ F2 pre(const Packed<V> (&win)[K], int i) const {
+    F2 s = bias.p[i];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-#pragma unroll
-    for (int j = 0; j < K; ++j) w[j][v] = param<T>(a.w, static_cast<long long>(c + v) * K + j, a.param_f32);
-    bias[v] = a.bias ? param<T>(a.bias, c + v, a.param_f32) : 0.f;
+    for (int j = 0; j < K; ++j) s = fma2(w[j].p[i], win[j].p[i], s);
+    return s;
   }
+};
+
+// The whole block loads the taps of its tx * V channels; buf: tx * (V * K + 1) floats.
+template <class T, int K, int V>
+__device__ __forceinline__ void load_taps(const pt_conv_args& a, int c0, float* buf, Taps<K, V>& taps) {
+  const int tx = static_cast<int>(blockDim.x), me = static_cast<int>(threadIdx.x);
+  const int n = min(tx * V, a.dim - c0) * K;
+  for (int i = static_cast<int>(threadIdx.y) * tx + me; i < n; i += kConvThreads)
+    buf[i / (V * K) * (V * K + 1) + i % (V * K)] = param<T>(a.w, static_cast<long long>(c0) * K + i, a.param_f32);
+  __syncthreads();
+  const bool in = c0 + me * V < a.dim;
+  const float* mine = buf + me * (V * K + 1);
+#pragma unroll
+  for (int i = 0; i < Packed<V>::N; ++i) {
+    const int v0 = 2 * i, v1 = 2 * i + 1 < V ? 2 * i + 1 : v0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) taps.w[j].p[i] = in ? pack2(mine[v0 * K + j], v1 > v0 ? mine[v1 * K + j] : 0.f) : 0;
+    const float b0 = in && a.bias ? param<T>(a.bias, c0 + me * V + v0, a.param_f32) : 0.f;
+    const float b1 = in && a.bias && v1 > v0 ? param<T>(a.bias, c0 + me * V + v1, a.param_f32) : 0.f;
+    taps.bias.p[i] = pack2(b0, b1);
+  }
+}
+
+__device__ __forceinline__ F2 sigmoid2(F2 v) {
+  const F2 m = mul2(v, pack2(-kLog2e, -kLog2e));
+  const F2 d = add2(pack2(ex2(lo2(m)), ex2(hi2(m))), pack2(1.f, 1.f));
+  return pack2(rcp(lo2(d)), rcp(hi2(d)));
 }
 
 template <class T, int K, int V>
 __global__ void __launch_bounds__(kConvThreads)
-    seq_conv_fwd_kernel(pt_conv_args a, int cblocks, int tblocks, int steps) {
-  constexpr int U = 4;  // steps whose loads are in flight together
+    seq_conv_fwd_kernel(pt_conv_args a, int cblocks, long long per) {
+  constexpr int U = kConvAhead;
+  extern __shared__ float tap_buf[];
   const int cb = static_cast<int>(blockIdx.x) % cblocks;
-  const int rest = static_cast<int>(blockIdx.x) / cblocks;
-  const int tb = rest % tblocks, b = rest / tblocks;
-  const int c = (cb * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * V;
+  const long long walker = static_cast<long long>(blockIdx.x / cblocks) * blockDim.y + threadIdx.y;
+  const int c0 = cb * static_cast<int>(blockDim.x) * V, c = c0 + static_cast<int>(threadIdx.x) * V;
+  Taps<K, V> taps;
+  load_taps<T, K, V>(a, c0, tap_buf, taps);
   if (c >= a.dim) return;
-  const int len = row_length(a.lengths, b, a.len);
-  ConvRow<T, K, V> row{static_cast<const T*>(a.x) + b * a.x_batch + c,
-                       a.state_in ? static_cast<const T*>(a.state_in) + static_cast<long long>(b) * (K - 1) * a.dim + c
-                                  : nullptr,
-                       a.x_step, a.dim, len};
-  if (K > 1 && a.state_out && tb == 0 && threadIdx.y == 0) {
-    T* out = static_cast<T*>(a.state_out) + static_cast<long long>(b) * (K - 1) * a.dim + c;
+  const long long walkers = static_cast<long long>(gridDim.x / cblocks) * blockDim.y;
+  if (K > 1 && a.state_out) {
+    for (long long b = walker; b < a.batch; b += walkers) {
+      const ConvRow<T, K, V> row = conv_row<T, K, V>(a, static_cast<int>(b), c);
+      T* out = static_cast<T*>(a.state_out) + b * (K - 1) * a.dim + c;
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) {
+        Pack<T, V> p;
+        row.load(p, row.len - (K - 1) + j);
+        p.store(out + static_cast<long long>(j) * a.dim, V, true);
+      }
+    }
+  }
+  const long long all = static_cast<long long>(a.batch) * a.len;
+  long long at = walker * per;
+  const long long end = min(at + per, all);
+  while (at < end) {
+    const int b = static_cast<int>(at / a.len), t0 = static_cast<int>(at % a.len);
+    const int t1 = static_cast<int>(min(static_cast<long long>(a.len), t0 + (end - at)));
+    const ConvRow<T, K, V> row = conv_row<T, K, V>(a, b, c);
+    Packed<V> win[K];  // win[j]: input at step t - K + 1 + j
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
       Pack<T, V> p;
-      row.load(p, len - (K - 1) + j);
-      p.store(out + static_cast<long long>(j) * a.dim, V, true);
+      row.load(p, t0 - (K - 1) + j);
+      win[j + 1].from(p);
     }
+    T* y = static_cast<T*>(a.y) + at * a.dim + c;
+    Pack<T, V> next[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) row.load(next[u], t0 + u);
+    for (int t = t0; t < t1; t += U) {
+      Pack<T, V> in[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) in[u] = next[u];
+      if (t + U < t1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) row.load(next[u], t + U + u);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
+        win[K - 1].from(in[u]);
+        Packed<V> s;
+#pragma unroll
+        for (int i = 0; i < Packed<V>::N; ++i) {
+          s.p[i] = taps.pre(win, i);
+          if (a.silu) s.p[i] = mul2(s.p[i], sigmoid2(s.p[i]));
+        }
+        if (t + u < t1) {
+          Pack<T, V> out;
+          s.to(out);
+          if (t + u >= row.len) out.zero();
+          out.store(y + static_cast<long long>(t + u - t0) * a.dim, V, true);
+        }
+      }
+    }
+    at += t1 - t0;
   }
-  const int t0 = (tb * static_cast<int>(blockDim.y) + static_cast<int>(threadIdx.y)) * steps;
-  const int t1 = min(t0 + steps, a.len);
-  if (t0 >= t1) return;
-  float w[K][V], bias[V];
-  conv_params<T, K, V>(a, c, w, bias);
-  float win[K][V];  // win[j]: input at step t - K + 1 + j
+}
+
+// Gradients of the steps [t0, t1) of row b: dx at those steps (at t0 = 0 the
+// state's too), and what they add to the taps' and the bias' gradients.
+template <class T, int K, int V>
+__device__ __forceinline__ void conv_bwd_stretch(const pt_conv_args& a, const Taps<K, V>& taps, int b, int t0, int t1, int c,
+                                                 Packed<V> (&dw)[K], Packed<V>& db) {
+  constexpr int U = kConvAhead;
+  const ConvRow<T, K, V> row = conv_row<T, K, V>(a, b, c);
+  const int len = row.len;
+  const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch + c;
+  T* dx = a.dx ? static_cast<T*>(a.dx) + static_cast<long long>(b) * a.len * a.dim + c : nullptr;
+  const long long s0 = static_cast<long long>(b) * (K - 1) * a.dim + c;
+  const T* dso = a.dstate_out ? static_cast<const T*>(a.dstate_out) + s0 : nullptr;
+  T* dsi = a.dstate_in ? static_cast<T*>(a.dstate_in) + s0 : nullptr;
+  Packed<V> win[K], gw[K];  // win[j]: input at step t - K + 1 + j; gw[j]: g at step t - j
+#pragma unroll
+  for (int j = 0; j < K; ++j) gw[j].zero();
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {
     Pack<T, V> p;
     row.load(p, t0 - (K - 1) + j);
-#pragma unroll
-    for (int v = 0; v < V; ++v) win[j + 1][v] = p.f(v);
+    win[j + 1].from(p);
   }
-  T* y = static_cast<T*>(a.y) + (static_cast<long long>(b) * a.len + t0) * a.dim + c;
-  for (int t = t0; t < t1; t += U) {
-    Pack<T, V> in[U];
+  const int first = t0 == 0 ? -(K - 1) : t0;  // first position whose gradient is written here
+  auto load_dy = [&](Pack<T, V>& p, int t) {
+    if (t < len)
+      p.load(dy + t * a.dy_step, V, true);
+    else
+      p.zero();
+  };
+  Pack<T, V> xn[U], gn[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) row.load(in[u], t + u);
+  for (int u = 0; u < U; ++u) row.load(xn[u], t0 + u), load_dy(gn[u], t0 + u);
+  for (int tt = t0; tt < t1 + K - 1; tt += U) {
+    Pack<T, V> xin[U], gin[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) xin[u] = xn[u], gin[u] = gn[u];
+    if (tt + U < t1 + K - 1) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) row.load(xn[u], tt + U + u), load_dy(gn[u], tt + U + u);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      Pack<T, V> out;
+      const int t = tt + u, pos = t - (K - 1);
+      Packed<V> g, s;
+      g.from(gin[u]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
+      for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
+      win[K - 1].from(xin[u]);
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) win[j][v] = win[j + 1][v];
-        win[K - 1][v] = in[u].f(v);
-        float s = bias[v];
+      for (int i = 0; i < Packed<V>::N; ++i) {
+        if (a.silu) {
+          const F2 one = pack2(1.f, 1.f), pre = taps.pre(win, i), sig = sigmoid2(pre);
+          // act' = sig (1 + pre (1 - sig))
+          const F2 rest = fma2(sig, pack2(-1.f, -1.f), one);
+          g.p[i] = mul2(g.p[i], mul2(sig, fma2(pre, rest, one)));
+        }
+        // Steps behind the row's end have no output; their window may hold anything.
+        if (t >= len) g.p[i] = 0;
+        if (t < t1 && t < len) {
 #pragma unroll
-        for (int j = 0; j < K; ++j) s = fmaf(w[j][v], win[j][v], s);
-        out.set(v, t + u < len ? (a.silu ? siluf(s) : s) : 0.f);
+          for (int j = 0; j < K; ++j) dw[j].p[i] = fma2(g.p[i], win[j].p[i], dw[j].p[i]);
+          db.p[i] = add2(db.p[i], g.p[i]);
+        }
+#pragma unroll
+        for (int j = K - 1; j > 0; --j) gw[j].p[i] = gw[j - 1].p[i];
+        gw[0].p[i] = g.p[i];
+        s.p[i] = 0;
+#pragma unroll
+        for (int j = 0; j < K; ++j) s.p[i] = fma2(taps.w[j].p[i], gw[j].p[i], s.p[i]);
       }
-      if (t + u < t1) out.store(y + static_cast<long long>(t + u - t0) * a.dim, V, true);
+      if (pos >= first && pos < t1) {
+        if (dso && pos >= len - (K - 1) && pos < len) {
+          Pack<T, V> more;
+          more.load(dso + static_cast<long long>(pos - (len - (K - 1))) * a.dim, V, true);
+          Packed<V> m;
+          m.from(more);
+#pragma unroll
+          for (int i = 0; i < Packed<V>::N; ++i) s.p[i] = add2(s.p[i], m.p[i]);
+        }
+        Pack<T, V> out;
+        s.to(out);
+        if (pos >= 0) {
+          if (dx) out.store(dx + static_cast<long long>(pos) * a.dim, V, true);
+        } else if (dsi) {
+          out.store(dsi + static_cast<long long>(pos + K - 1) * a.dim, V, true);
+        }
+      }
     }
   }
 }
 
-// Work item i of a block's list is batch row i / tblocks, steps from
-// (i % tblocks) * kConvBwdTy * steps on; the dw of all its items stay in registers.
 template <class T, int K, int V>
 __global__ void __launch_bounds__(kConvThreads)
-    seq_conv_bwd_kernel(pt_conv_args a, float* part, int cblocks, int tblocks, int steps, int chunks) {
-  __shared__ float red[kConvBwdTy][kConvBwdTx * V];
-  const int tx = static_cast<int>(threadIdx.x), ty = static_cast<int>(threadIdx.y);
+    seq_conv_bwd_kernel(pt_conv_args a, float* part, int cblocks, long long per) {
+  extern __shared__ float tap_buf[];
+  const int tx = static_cast<int>(blockDim.x), ty = static_cast<int>(blockDim.y);
+  const int x = static_cast<int>(threadIdx.x), y = static_cast<int>(threadIdx.y);
   const int cb = static_cast<int>(blockIdx.x) % cblocks, chunk = static_cast<int>(blockIdx.x) / cblocks;
-  const int c = (cb * kConvBwdTx + tx) * V;
-  const bool in = c < a.dim;
-  float w[K][V], bias[V], dw[K][V], db[V];
+  const int c0 = cb * tx * V, c = c0 + x * V;
+  Taps<K, V> taps;
+  load_taps<T, K, V>(a, c0, tap_buf, taps);
+  Packed<V> dw[K], db;
+  db.zero();
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    db[v] = 0.f;
-#pragma unroll
-    for (int j = 0; j < K; ++j) dw[j][v] = 0.f;
-  }
-  if (in) {
-    conv_params<T, K, V>(a, c, w, bias);
-    const long long items = static_cast<long long>(a.batch) * tblocks;
-    for (long long item = chunk; item < items; item += chunks) {
-      const int b = static_cast<int>(item / tblocks), tb = static_cast<int>(item % tblocks);
-      const int len = row_length(a.lengths, b, a.len);
-      const int t0 = (tb * kConvBwdTy + ty) * steps, t1 = min(t0 + steps, a.len);
-      if (t0 >= t1 && !(t0 == 0)) continue;
-      ConvRow<T, K, V> row{
-          static_cast<const T*>(a.x) + b * a.x_batch + c,
-          a.state_in ? static_cast<const T*>(a.state_in) + static_cast<long long>(b) * (K - 1) * a.dim + c : nullptr,
-          a.x_step, a.dim, len};
-      const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch + c;
-      T* dx = a.dx ? static_cast<T*>(a.dx) + static_cast<long long>(b) * a.len * a.dim + c : nullptr;
-      const T* dso = a.dstate_out
-                         ? static_cast<const T*>(a.dstate_out) + static_cast<long long>(b) * (K - 1) * a.dim + c
-                         : nullptr;
-      T* dsi = a.dstate_in ? static_cast<T*>(a.dstate_in) + static_cast<long long>(b) * (K - 1) * a.dim + c : nullptr;
-      float win[K][V], gw[K][V];  // gw[j]: g at step t - j
-#pragma unroll
-      for (int j = 0; j < K; ++j)
-#pragma unroll
-        for (int v = 0; v < V; ++v) gw[j][v] = 0.f;
-#pragma unroll
-      for (int j = 0; j < K - 1; ++j) {
-        Pack<T, V> p;
-        row.load(p, t0 - (K - 1) + j);
-#pragma unroll
-        for (int v = 0; v < V; ++v) win[j + 1][v] = p.f(v);
-      }
-      const int first = t0 == 0 ? -(K - 1) : t0;  // first position whose gradient this thread writes
-      constexpr int U = 4;
-      for (int tt = t0; tt < t1 + K - 1; tt += U) {
-        Pack<T, V> xin[U], gin[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          row.load(xin[u], tt + u);
-          if (tt + u < len)
-            gin[u].load(dy + (tt + u) * a.dy_step, V, true);
-          else
-            gin[u].zero();
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int t = tt + u, pos = t - (K - 1);
-          Pack<T, V> out;
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-#pragma unroll
-            for (int j = 0; j < K - 1; ++j) win[j][v] = win[j + 1][v];
-            win[K - 1][v] = xin[u].f(v);
-            float g = gin[u].f(v);
-            if (a.silu) {
-              float pre = bias[v];
-#pragma unroll
-              for (int j = 0; j < K; ++j) pre = fmaf(w[j][v], win[j][v], pre);
-              g *= silu_grad(pre, sigmoidf(pre));
-            }
-            // Steps behind the row's end have no output; their window may hold anything.
-            g = t < len ? g : 0.f;
-            if (t < t1 && t < len) {
-#pragma unroll
-              for (int j = 0; j < K; ++j) dw[j][v] = fmaf(g, win[j][v], dw[j][v]);
-              db[v] += g;
-            }
-#pragma unroll
-            for (int j = K - 1; j > 0; --j) gw[j][v] = gw[j - 1][v];
-            gw[0][v] = g;
-            float s = 0.f;
-#pragma unroll
-            for (int j = 0; j < K; ++j) s = fmaf(w[j][v], gw[j][v], s);
-            if (dso && pos >= len - (K - 1) && pos < len)
-              s += to_f<T>(dso[static_cast<long long>(pos - (len - (K - 1))) * a.dim + v]);
-            out.set(v, s);
-          }
-          if (pos >= first && pos < t1) {
-            if (pos >= 0) {
-              if (dx) out.store(dx + static_cast<long long>(pos) * a.dim, V, true);
-            } else if (dsi) {
-              out.store(dsi + static_cast<long long>(pos + K - 1) * a.dim, V, true);
-            }
-          }
-        }
+  for (int j = 0; j < K; ++j) dw[j].zero();
+  if (c < a.dim) {
+    const long long walker = static_cast<long long>(chunk) * ty + y;
+    if (a.len == 0) {
+      // No steps: what the final state's gradient gives to the initial state.
+      for (long long b = walker; b < a.batch; b += static_cast<long long>(gridDim.x / cblocks) * ty)
+        conv_bwd_stretch<T, K, V>(a, taps, static_cast<int>(b), 0, 0, c, dw, db);
+    } else {
+      const long long all = static_cast<long long>(a.batch) * a.len;
+      long long at = walker * per;
+      const long long end = min(at + per, all);
+      while (at < end) {
+        const int b = static_cast<int>(at / a.len), t0 = static_cast<int>(at % a.len);
+        const int t1 = static_cast<int>(min(static_cast<long long>(a.len), t0 + (end - at)));
+        conv_bwd_stretch<T, K, V>(a, taps, b, t0, t1, c, dw, db);
+        at += t1 - t0;
       }
     }
   }
@@ -227,16 +321,16 @@ __global__ void __launch_bounds__(kConvThreads)
   float* mine = part + static_cast<long long>(chunk) * a.dim * (K + 1);
 #pragma unroll
   for (int j = 0; j <= K; ++j) {
+    const Packed<V>& from = j < K ? dw[j < K ? j : 0] : db;
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < V; ++v) red[ty][tx * V + v] = j < K ? dw[j < K ? j : 0][v] : db[v];
+    for (int v = 0; v < V; ++v) tap_buf[(y * tx + x) * V + v] = v & 1 ? hi2(from.p[v / 2]) : lo2(from.p[v / 2]);
     __syncthreads();
-    for (int i = ty * kConvBwdTx + tx; i < kConvBwdTx * V; i += kConvThreads) {
-      const int d = cb * kConvBwdTx * V + i;
+    for (int i = y * tx + x; i < tx * V; i += kConvThreads) {
+      const int d = c0 + i;
       if (d < a.dim) {
         float s = 0.f;
-#pragma unroll
-        for (int r = 0; r < kConvBwdTy; ++r) s += red[r][i];
+        for (int r = 0; r < ty; ++r) s += tap_buf[r * tx * V + i];
         mine[j < K ? static_cast<long long>(d) * K + j : static_cast<long long>(a.dim) * K + d] = s;
       }
     }
@@ -244,11 +338,27 @@ __global__ void __launch_bounds__(kConvThreads)
 }
 
 template <class T, int K, int V>
-__global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_args a, int cblocks, unsigned* err) {
+__global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_args a, int cblocks, bool wide, unsigned* err) {
   const int cb = static_cast<int>(blockIdx.x) % cblocks, b = static_cast<int>(blockIdx.x) / cblocks;
-  const int slot = a.slots ? slot_of(a.slots, b, a.cache_rows, err, static_cast<int>(threadIdx.x), kConvThreads) : b;
   const int c = (cb * kConvThreads + static_cast<int>(threadIdx.x)) * V;
-  if (c >= a.dim) return;
+  const bool in = c < a.dim;
+  // What does not depend on the slot is under way while the slot is looked up.
+  Pack<T, V> win[K];
+  Pack<float, V * K> w;
+  Pack<float, V> bias;
+  if (in) {
+    win[K - 1].load(static_cast<const T*>(a.x) + b * a.x_batch + c, V, true);
+    if (a.param_f32) {
+      w.load(static_cast<const float*>(a.w) + static_cast<long long>(c) * K, V * K, wide);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V * K; ++i) w.v[i] = param<T>(a.w, static_cast<long long>(c) * K + i, false);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias.v[v] = a.bias ? param<T>(a.bias, c + v, a.param_f32) : 0.f;
+  }
+  const int slot = a.slots ? slot_of(a.slots, b, a.cache_rows, err, static_cast<int>(threadIdx.x), kConvThreads) : b;
+  if (!in) return;
   T* y = static_cast<T*>(a.y) + static_cast<long long>(b) * a.dim + c;
   Pack<T, V> out;
   if (slot < 0) {
@@ -257,31 +367,27 @@ __global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_arg
     return;
   }
   T* state = static_cast<T*>(a.state_out) + static_cast<long long>(slot) * a.state_row + c;
-  Pack<T, V> in[K];
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) {
+    // Plain loads, not the read-only ones: the cache is written below.
     const T* p = state + static_cast<long long>(j) * a.dim;
-    // Plain loads: the cache is written below.
-    if constexpr (V * sizeof(T) == 16) {
-      *reinterpret_cast<uint4*>(in[j].v) = *reinterpret_cast<const uint4*>(p);
+    if constexpr (V == 2 && sizeof(T) == 2) {
+      *reinterpret_cast<unsigned*>(win[j].v) = *reinterpret_cast<const unsigned*>(p);
     } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) in[j].v[v] = p[v];
+      for (int v = 0; v < V; ++v) win[j].v[v] = p[v];
     }
   }
-  in[K - 1].load(static_cast<const T*>(a.x) + b * a.x_batch + c, V, true);
-  float w[K][V], bias[V];
-  conv_params<T, K, V>(a, c, w, bias);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    float s = bias[v];
+    float s = bias.v[v];
 #pragma unroll
-    for (int j = 0; j < K; ++j) s = fmaf(w[j][v], in[j].f(v), s);
-    out.set(v, a.silu ? siluf(s) : s);
+    for (int j = 0; j < K; ++j) s = fmaf(w.v[v * K + j], win[j].f(v), s);
+    out.set(v, a.silu ? s * lo2(sigmoid2(pack2(s, s))) : s);
   }
   out.store(y, V, true);
 #pragma unroll
-  for (int j = 0; j < K - 1; ++j) in[j + 1].store(state + static_cast<long long>(j) * a.dim, V, true);
+  for (int j = 0; j < K - 1; ++j) win[j + 1].store(state + static_cast<long long>(j) * a.dim, V, true);
 }
 
 // ---------------------------------------------------------------- host side
@@ -316,8 +422,10 @@ cudaError_t by_width_taps(int v, int k, F&& fn) {
     }
   };
   if (v == 1) return taps(std::integral_constant<int, 1>());
-  if (v == 2) return taps(std::integral_constant<int, 2>());
-  return taps(std::integral_constant<int, VMAX>());
+  if constexpr (VMAX > 2) {
+    if (v > 2) return taps(std::integral_constant<int, VMAX>());
+  }
+  return taps(std::integral_constant<int, 2>());
 }
 
 template <class T>
@@ -325,39 +433,48 @@ constexpr int conv_word = 16 / static_cast<int>(sizeof(T));  // forward: 16 byte
 template <class T>
 constexpr int conv_bwd_word = sizeof(T) == 4 ? 4 : 4;  // backward: four channels (registers: five arrays of taps)
 
-template <class T>
-ConvBwdPlan conv_bwd_plan(const pt_conv_args& a, int sm_count) {
-  ConvBwdPlan p;
-  p.v = conv_width(a, sizeof(T), conv_bwd_word<T>);
-  p.cblocks = static_cast<int>(cdiv(a.dim, kConvBwdTx * p.v));
-  // As many steps per thread as leave eight blocks per SM, at least 8.
-  p.steps = 64;
-  while (p.steps > 8 && static_cast<long long>(p.cblocks) * a.batch * cdiv(a.len, p.steps * kConvBwdTy) < 8 * sm_count)
-    p.steps /= 2;
-  p.tblocks = static_cast<int>(cdiv(a.len > 0 ? a.len : 1, p.steps * kConvBwdTy));
-  const long long items = static_cast<long long>(a.batch) * p.tblocks;
-  const long long most = cdiv(8LL * sm_count, p.cblocks);
-  p.chunks = static_cast<int>(items < most ? items : most);
+// Threads along the channels (the rest of the block's 128 along the steps), and
+// how many stretches of how many steps: `want` threads in all, at least `least`
+// steps each, so that the overlap stays small.
+struct ConvCut {
+  int tx, ty, cblocks;
+  long long per, walkers;
+};
+inline ConvCut conv_cut(const pt_conv_args& a, int v, long long want, int least) {
+  ConvCut p;
+  const long long groups = cdiv(a.dim, v), all = static_cast<long long>(a.batch) * a.len;
+  p.tx = 32;
+  while (p.tx < kConvThreads && p.tx < groups) p.tx *= 2;
+  p.ty = kConvThreads / p.tx;
+  p.cblocks = static_cast<int>(cdiv(groups, p.tx));
+  const long long most = cdiv(want, static_cast<long long>(p.cblocks) * p.tx);
+  p.per = cdiv(all > 0 ? all : 1, most);
+  if (p.per < least) p.per = least;
+  p.walkers = cdiv(all > 0 ? all : 1, p.per);
   return p;
 }
 
 template <class T>
-cudaError_t conv_fwd(const pt_conv_args& a, cudaStream_t stream) {
+ConvBwdPlan conv_bwd_plan(const pt_conv_args& a, int sm_count) {
+  ConvBwdPlan p;
+  p.v = conv_width(a, sizeof(T), conv_bwd_word<T>);
+  // Four blocks' worth of threads per SM.
+  const ConvCut c = conv_cut(a, p.v, 512LL * sm_count, 24);
+  p.tx = c.tx, p.cblocks = c.cblocks, p.per = c.per;
+  p.chunks = static_cast<int>(cdiv(c.walkers, c.ty));
+  return p;
+}
+
+template <class T>
+cudaError_t conv_fwd(const pt_conv_args& a, int sm_count, cudaStream_t stream) {
   const int v = conv_width(a, sizeof(T), conv_word<T>);
-  const int groups = static_cast<int>(cdiv(a.dim, v));
-  int tx = 32;
-  while (tx < kConvThreads && tx < groups) tx *= 2;
-  const int ty = kConvThreads / tx;
-  const int cblocks = static_cast<int>(cdiv(groups, tx));
-  int steps = 32;
-  while (steps > 4 && static_cast<long long>(cblocks) * a.batch * cdiv(a.len, static_cast<long long>(steps) * ty) < 1184)
-    steps /= 2;
-  const int tblocks = static_cast<int>(cdiv(a.len > 0 ? a.len : 1, static_cast<long long>(steps) * ty));
-  const long long grid = static_cast<long long>(cblocks) * tblocks * a.batch;
+  const ConvCut p = conv_cut(a, v, 2048LL * sm_count, 8);
+  const long long grid = p.cblocks * cdiv(p.walkers, p.ty);
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   return by_width_taps<conv_word<T>>(v, a.taps, [&](auto vc, auto kc) {
-    seq_conv_fwd_kernel<T, decltype(kc)::value, decltype(vc)::value>
-        <<<static_cast<unsigned>(grid), dim3(tx, ty), 0, stream>>>(a, cblocks, tblocks, steps);
+    constexpr int V = decltype(vc)::value, K = decltype(kc)::value;
+    seq_conv_fwd_kernel<T, K, V><<<static_cast<unsigned>(grid), dim3(p.tx, p.ty), sizeof(float) * p.tx * (V * K + 1), stream>>>(
+        a, p.cblocks, p.per);
     return cudaGetLastError();
   });
 }
@@ -365,10 +482,14 @@ cudaError_t conv_fwd(const pt_conv_args& a, cudaStream_t stream) {
 template <class T>
 cudaError_t conv_bwd(const pt_conv_args& a, float* ws, int sm_count, cudaStream_t stream) {
   const ConvBwdPlan p = conv_bwd_plan<T>(a, sm_count);
+  const long long grid = static_cast<long long>(p.cblocks) * p.chunks;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   cudaError_t e = by_width_taps<conv_bwd_word<T>>(p.v, a.taps, [&](auto vc, auto kc) {
-    seq_conv_bwd_kernel<T, decltype(kc)::value, decltype(vc)::value>
-        <<<static_cast<unsigned>(p.cblocks * p.chunks), dim3(kConvBwdTx, kConvBwdTy), 0, stream>>>(
-            a, ws, p.cblocks, p.tblocks, p.steps, p.chunks);
+    constexpr int V = decltype(vc)::value, K = decltype(kc)::value;
+    const int floats = p.tx * (V * K + 1) > kConvThreads * V ? p.tx * (V * K + 1) : kConvThreads * V;
+    seq_conv_bwd_kernel<T, K, V>
+        <<<static_cast<unsigned>(grid), dim3(p.tx, kConvThreads / p.tx), sizeof(float) * floats, stream>>>(
+            a, ws, p.cblocks, p.per);
     return cudaGetLastError();
   });
   if (e != cudaSuccess) return e;
@@ -381,13 +502,15 @@ cudaError_t conv_bwd(const pt_conv_args& a, float* ws, int sm_count, cudaStream_
 
 template <class T>
 cudaError_t conv_step(const pt_conv_args& a, unsigned* err, cudaStream_t stream) {
-  const int v = conv_width(a, sizeof(T), conv_word<T>);
+  // Two channels per thread: a call is short, so many threads with little each.
+  const int v = conv_width(a, sizeof(T), 2);
   const int cblocks = static_cast<int>(cdiv(a.dim, kConvThreads * v));
   const long long grid = static_cast<long long>(cblocks) * a.batch;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  return by_width_taps<conv_word<T>>(v, a.taps, [&](auto vc, auto kc) {
-    seq_conv_step_kernel<T, decltype(kc)::value, decltype(vc)::value>
-        <<<static_cast<unsigned>(grid), kConvThreads, 0, stream>>>(a, cblocks, err);
+  return by_width_taps<2>(v, a.taps, [&](auto vc, auto kc) {
+    constexpr int V = decltype(vc)::value, K = decltype(kc)::value;
+    const bool wide = aligned(a.w, Pack<float, V * K>::kWord);
+    seq_conv_step_kernel<T, K, V><<<static_cast<unsigned>(grid), kConvThreads, 0, stream>>>(a, cblocks, wide, err);
     return cudaGetLastError();
   });
 }

@@ -3,7 +3,7 @@
 
 namespace pt {
 namespace seq {
-template cudaError_t conv_fwd<__half>(const pt_conv_args&, cudaStream_t);
+template cudaError_t conv_fwd<__half>(const pt_conv_args&, int, cudaStream_t);
 template cudaError_t conv_bwd<__half>(const pt_conv_args&, float*, int, cudaStream_t);
 template cudaError_t conv_step<__half>(const pt_conv_args&, unsigned*, cudaStream_t);
 template ConvBwdPlan conv_bwd_plan<__half>(const pt_conv_args&, int);

@@ -41,6 +41,9 @@ constexpr int kSub = 4;    // backward: steps whose states and decays are in reg
 // A block: 4 warps that scan, 4 warps that stage.
 constexpr int kScanners = 128, kStagers = 128, kBlock = kScanners + kStagers;
 constexpr int kScanWarps = kScanners / 32;
+// Backward, registers per thread: two blocks per SM are launched with 128 for
+// each thread; the scanners take 40 of the stagers'.
+constexpr int kScannerRegs = 168, kStagerRegs = 88;
 
 template <int S>
 struct ScanShape {
@@ -557,40 +560,37 @@ __global__ void __launch_bounds__(kBlock, 2)
   auto tile_of = [&](int k) { return t0 + (tiles - 1 - k) * kTile; };
 
   if (tid >= kScanners) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kStagerRegs));
     const Stager<S> me(tid - kScanners, at.c0, at.nch);
     float accD[P::kE] = {}, accb[P::kE] = {};
     for (int b = chunk; b < a.batch; b += dm.row_chunks) {
       const int len = scan_row_length(a, b);
-      struct Raw {
-        Pack<T, P::kE> dt, x, z, dy;
-      } next, last;  // of the tile to convert, of the tile whose gradients are to be written
-      StateRow<T, S> rowB, rowC;
-      auto load = [&](int k, Raw& r) {
+      // A tile takes the scanners far longer than a trip to memory, so nothing is fetched ahead and few registers do.
+      Pack<T, P::kE> dt, x, z, dy;
+      auto load = [&](int k) {
         const int t = tile_of(k) + me.tr;
         if (t < len && t < t1) {
-          r.dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
-          r.x.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
-          r.dy.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + me.c, me.n, dm.wide & 8);
-          if (a.z) r.z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
+          dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
+          x.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
+          dy.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + me.c, me.n, dm.wide & 8);
+          if (a.z) z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
         }
-      };
-      auto load_next = [&](int k) {
-        load(k, next);
-        const int t = tile_of(k) + me.tr;
-        const bool live = t < len && t < t1;
-        rowB.load(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live, me.pr);
-        rowC.load(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live, me.pr);
       };
       auto convert = [&](int k) {
         const int t = tile_of(k) + me.tr;
+        const bool live = t < len && t < t1;
+        load(k);
+        StateRow<T, S> rowB, rowC;
+        rowB.load(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live, me.pr);
+        rowC.load(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live, me.pr);
         float d[P::kE] = {}, v[P::kE] = {}, w[P::kE] = {};
-        if (t < len && t < t1) {
+        if (live) {
 #pragma unroll
           for (int i = 0; i < P::kE; ++i) {
-            const float raw = next.dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f);
+            const float raw = dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f);
             d[i] = a.dt_softplus ? softplusf(raw) : raw;
-            v[i] = d[i] * next.x.f(i);
-            w[i] = a.z ? next.dy.f(i) * siluf(next.z.f(i)) : next.dy.f(i);
+            v[i] = d[i] * x.f(i);
+            w[i] = a.z ? dy.f(i) * siluf(z.f(i)) : dy.f(i);
           }
         }
         put_floats<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
@@ -602,6 +602,7 @@ __global__ void __launch_bounds__(kBlock, 2)
       auto finish = [&](int k) {
         const int tile = tile_of(k), t = tile + me.tr, st = k & 1;
         if (t < t1) {
+          load(k);
           Pack<T, P::kE> ox, odt, oz;
           ox.zero(), odt.zero(), oz.zero();
           if (t < len) {
@@ -612,20 +613,20 @@ __global__ void __launch_bounds__(kBlock, 2)
             get_floats<P::kE>(&sm.w[st][me.tr][me.col], y);
 #pragma unroll
             for (int i = 0; i < P::kE; ++i) {
-              const float x = last.x.f(i), dy = last.dy.f(i);
+              const float xv = x.f(i), dyv = dy.f(i);
               const float Dv = a.D && i < me.n ? __ldg(a.D + me.c + i) : 0.f;
-              float w = dy;
+              float w = dyv;
               if (a.z) {
-                const float z = last.z.f(i), s = sigmoidf(z);
-                w *= z * s;
-                oz.set(i, dy * (a.D ? fmaf(Dv, x, y[i]) : y[i]) * silu_grad(z, s));
+                const float zv = z.f(i), s = sigmoidf(zv);
+                w *= zv * s;
+                oz.set(i, dyv * (a.D ? fmaf(Dv, xv, y[i]) : y[i]) * silu_grad(zv, s));
               }
-              float gd = fmaf(gB[i], x, gA[i] * kLn2);
+              float gd = fmaf(gB[i], xv, gA[i] * kLn2);
               if (a.dt_softplus)
-                gd *= sigmoidf(last.dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f));
+                gd *= sigmoidf(dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f));
               ox.set(i, a.D ? fmaf(Dv, w, gB[i] * d[i]) : gB[i] * d[i]);
               odt.set(i, gd);
-              accD[i] = fmaf(w, x, accD[i]);
+              accD[i] = fmaf(w, xv, accD[i]);
               accb[i] += gd;
             }
           }
@@ -650,22 +651,11 @@ __global__ void __launch_bounds__(kBlock, 2)
           }
         }
       };
-      if (tiles > 0) {
-        load_next(0);
-        convert(0);
-        if (tiles > 1) load_next(1);
-        load(0, last);
-      }
+      if (tiles > 0) convert(0);
       meet();
       for (int k = 0; k < tiles; ++k) {
-        if (k > 0) {
-          finish(k - 1);
-          load(k, last);
-        }
-        if (k + 1 < tiles) {
-          convert(k + 1);
-          if (k + 2 < tiles) load_next(k + 2);
-        }
+        if (k > 0) finish(k - 1);
+        if (k + 1 < tiles) convert(k + 1);
         meet();
       }
       if (tiles > 0) finish(tiles - 1);
@@ -684,6 +674,7 @@ __global__ void __launch_bounds__(kBlock, 2)
     return;
   }
 
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kScannerRegs));
   const Scanner<S> me(tid, at.c0, at.nch);
   Quad A2;
   load_rates(a, me, A2);
@@ -743,7 +734,7 @@ __global__ void __launch_bounds__(kBlock, 2)
           *reinterpret_cast<ulonglong2*>(&sm.start[sub][c][tid]) = make_ulonglong2(h[c][0], h[c][1]);
       }
       Quad dA = {};
-#pragma unroll 1
+#pragma unroll 2
       for (int sub = kTile / kSub - 1; sub >= 0; --sub) {
         const int i0 = sub * kSub;
         F2 hs[kSub + 1][2][2], as[kSub][2][2];  // hs[i]: the state before step i0 + i
