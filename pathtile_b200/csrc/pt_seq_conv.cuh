@@ -25,7 +25,18 @@ namespace pt {
 namespace seq {
 
 constexpr int kConvThreads = 128;
-constexpr int kConvAhead = 4;  // steps whose loads are under way together
+
+// Blocks per SM that the registers are kept down for, and steps whose loads are
+// under way together.  One wave of long stretches beats several waves of short
+// ones (8 x 2048 x 4096 bf16, 4 taps: forward 60 against 69 us with four waves;
+// backward 129 us, 200 us at the 146 registers that it would take by itself).
+// Narrow words (rows that are not aligned) need more threads and steps for the
+// same bytes on their way.
+template <int V>
+constexpr int kConvFwdBlocks = V > 2 ? 4 : 8;
+template <int V>
+constexpr int kConvFwdAhead = V > 2 ? 4 : 8;
+constexpr int kConvBwdBlocks = 4, kConvBwdAhead = 4;
 
 __device__ __forceinline__ int row_length(const int* lengths, int b, int len) {
   if (!lengths) return len;
@@ -122,9 +133,9 @@ __device__ __forceinline__ F2 sigmoid2(F2 v) {
 }
 
 template <class T, int K, int V>
-__global__ void __launch_bounds__(kConvThreads)
+__global__ void __launch_bounds__(kConvThreads, kConvFwdBlocks<V>)
     seq_conv_fwd_kernel(pt_conv_args a, int cblocks, long long per) {
-  constexpr int U = kConvAhead;
+  constexpr int U = kConvFwdAhead<V>;
   extern __shared__ float tap_buf[];
   const int cb = static_cast<int>(blockIdx.x) % cblocks;
   const long long walker = static_cast<long long>(blockIdx.x / cblocks) * blockDim.y + threadIdx.y;
@@ -199,7 +210,7 @@ __global__ void __launch_bounds__(kConvThreads)
 template <class T, int K, int V>
 __device__ __forceinline__ void conv_bwd_stretch(const pt_conv_args& a, const Taps<K, V>& taps, int b, int t0, int t1, int c,
                                                  Packed<V> (&dw)[K], Packed<V>& db) {
-  constexpr int U = kConvAhead;
+  constexpr int U = kConvBwdAhead;
   const ConvRow<T, K, V> row = conv_row<T, K, V>(a, b, c);
   const int len = row.len;
   const T* dy = static_cast<const T*>(a.dy) + b * a.dy_batch + c;
@@ -286,7 +297,7 @@ __device__ __forceinline__ void conv_bwd_stretch(const pt_conv_args& a, const Ta
 }
 
 template <class T, int K, int V>
-__global__ void __launch_bounds__(kConvThreads)
+__global__ void __launch_bounds__(kConvThreads, kConvBwdBlocks)
     seq_conv_bwd_kernel(pt_conv_args a, float* part, int cblocks, long long per) {
   extern __shared__ float tap_buf[];
   const int tx = static_cast<int>(blockDim.x), ty = static_cast<int>(blockDim.y);
@@ -391,11 +402,15 @@ __global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_arg
 }
 
 // ---------------------------------------------------------------- host side
+// Widest words; more than four taps leave registers for two channels only.
+constexpr int kConvWideTaps = 4;
+
 // Whether every row that `ptr` leads to starts on a word of V elements.
 inline bool conv_wide(const void* ptr, long long s0, long long s1, int v, size_t e) {
   return !ptr || (aligned(ptr, v * e) && s0 % v == 0 && s1 % v == 0);
 }
 inline int conv_width(const pt_conv_args& a, size_t e, int most) {
+  if (a.taps > kConvWideTaps && most > 2) most = 2;
   for (int v = most; v > 1; v = v > 2 ? 2 : 1) {
     if (a.dim % v == 0 && conv_wide(a.x, a.x_batch, a.x_step, v, e) && conv_wide(a.dy, a.dy_batch, a.dy_step, v, e) &&
         conv_wide(a.state_in, 0, 0, v, e) && conv_wide(a.state_out, a.state_row, 0, v, e) && conv_wide(a.y, 0, 0, v, e) &&
@@ -410,16 +425,22 @@ template <int VMAX, class F>
 cudaError_t by_width_taps(int v, int k, F&& fn) {
   auto taps = [&](auto vc) -> cudaError_t {
     switch (k) {
-      case 1: return fn(vc, std::integral_constant<int, 1>());
+            case 1: return fn(vc, std::integral_constant<int, 1>());
       case 2: return fn(vc, std::integral_constant<int, 2>());
       case 3: return fn(vc, std::integral_constant<int, 3>());
-      case 4: return fn(vc, std::integral_constant<int, 4>());
-      case 5: return fn(vc, std::integral_constant<int, 5>());
-      case 6: return fn(vc, std::integral_constant<int, 6>());
-      case 7: return fn(vc, std::integral_constant<int, 7>());
-      case 8: return fn(vc, std::integral_constant<int, 8>());
-      default: return cudaErrorInvalidValue;
+            case 4: return fn(vc, std::integral_constant<int, 4>());
+      default: break;
     }
+    if constexpr (decltype(vc)::value <= 2) {
+      switch (k) {
+        case 5: return fn(vc, std::integral_constant<int, 5>());
+        case 6: return fn(vc, std::integral_constant<int, 6>());
+        case 7: return fn(vc, std::integral_constant<int, 7>());
+        case 8: return fn(vc, std::integral_constant<int, 8>());
+        default: break;
+      }
+    }
+    return cudaErrorInvalidValue;
   };
   if (v == 1) return taps(std::integral_constant<int, 1>());
   if constexpr (VMAX > 2) {
@@ -431,7 +452,7 @@ cudaError_t by_width_taps(int v, int k, F&& fn) {
 template <class T>
 constexpr int conv_word = 16 / static_cast<int>(sizeof(T));  // forward: 16 bytes
 template <class T>
-constexpr int conv_bwd_word = sizeof(T) == 4 ? 4 : 4;  // backward: four channels (registers: five arrays of taps)
+constexpr int conv_bwd_word = sizeof(T) == 4 ? 2 : 4;
 
 // Threads along the channels (the rest of the block's 128 along the steps), and
 // how many stretches of how many steps: `want` threads in all, at least `least`
@@ -458,8 +479,7 @@ template <class T>
 ConvBwdPlan conv_bwd_plan(const pt_conv_args& a, int sm_count) {
   ConvBwdPlan p;
   p.v = conv_width(a, sizeof(T), conv_bwd_word<T>);
-  // Four blocks' worth of threads per SM.
-  const ConvCut c = conv_cut(a, p.v, 512LL * sm_count, 24);
+  const ConvCut c = conv_cut(a, p.v, kConvBwdBlocks * static_cast<long long>(kConvThreads) * sm_count, 24);
   p.tx = c.tx, p.cblocks = c.cblocks, p.per = c.per;
   p.chunks = static_cast<int>(cdiv(c.walkers, c.ty));
   return p;
@@ -468,7 +488,7 @@ ConvBwdPlan conv_bwd_plan(const pt_conv_args& a, int sm_count) {
 template <class T>
 cudaError_t conv_fwd(const pt_conv_args& a, int sm_count, cudaStream_t stream) {
   const int v = conv_width(a, sizeof(T), conv_word<T>);
-  const ConvCut p = conv_cut(a, v, 2048LL * sm_count, 8);
+  const ConvCut p = conv_cut(a, v, (v > 2 ? kConvFwdBlocks<4> : kConvFwdBlocks<2>) * static_cast<long long>(kConvThreads) * sm_count, 8);
   const long long grid = p.cblocks * cdiv(p.walkers, p.ty);
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   return by_width_taps<conv_word<T>>(v, a.taps, [&](auto vc, auto kc) {
