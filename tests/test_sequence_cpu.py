@@ -10,7 +10,7 @@ import torch
 
 import pathtile_b200 as pt
 from oracle import sequence as ref
-from pathtile_b200 import _lib, sequence
+from pathtile_b200 import _lib
 
 FAKE = 0x10000  # aligned, never dereferenced: checks fail before any CUDA call
 NULL = None
@@ -134,49 +134,16 @@ def test_the_structs_have_the_headers_layout(tmp_path):
 
 
 # ---------------------------------------------------------------- Python checks
-def test_only_cuda_tensors_of_the_supported_types():
+def test_only_cuda_tensors_of_the_supported_types(native_lib):
     x, w = torch.zeros(2, 4, 8), torch.zeros(8, 4)
     for call in (lambda: pt.causal_conv(x, w), lambda: pt.causal_conv_step(torch.zeros(2, 3, 8), x[:, 0], w),
                  lambda: pt.selective_scan(x, x, w, x, x), lambda: pt.fused_norm(x, torch.zeros(8))):
         with pytest.raises(ValueError, match="CUDA"):
             call()
-    for call in (lambda: pt.causal_conv(3, w), lambda: pt.selective_scan([1.0], x, w, x, x), lambda: pt.fused_norm(None, w)):
+    for call in (lambda: pt.causal_conv(3, w), lambda: pt.selective_scan([1.0], x, w, x, x), lambda: pt.fused_norm(None, w),
+                 lambda: pt.causal_conv(x, w, silu="yes"), lambda: pt.selective_scan(x, x, w, x, x, lengths=[1, 2])):
         with pytest.raises(TypeError):
             call()
-
-
-def test_a_cache_must_be_updatable_in_place():
-    dev, f32 = torch.device("cpu"), torch.float32
-    whole = torch.zeros(5, 6, 4)
-    assert sequence._cache(whole, "state", (6, 4), f32, dev) == (5, 24)
-    layers = torch.zeros(5, 3, 6, 4)
-    assert sequence._cache(layers[:, 1], "state", (6, 4), f32, dev) == (5, 72)  # one layer of a cache of three
-    for bad in (whole.transpose(1, 2).contiguous().transpose(1, 2), whole[:1].expand(5, 6, 4), whole.double(), whole[0],
-                torch.zeros(5, 4, 6), whole.to("meta")):
-        with pytest.raises(ValueError):
-            sequence._cache(bad, "state", (6, 4), f32, dev)
-    with pytest.raises(TypeError):
-        sequence._cache(None, "state", (6, 4), f32, dev)
-
-
-def test_slots_are_checked():
-    dev = torch.device("cpu")
-    assert sequence._slots(None, 4, 4, "state", dev) is None
-    with pytest.raises(ValueError, match="slots"):
-        sequence._slots(None, 4, 7, "state", dev)
-    good = torch.arange(4, dtype=torch.int32)
-    assert sequence._slots(good, 4, 7, "state", dev) is good
-    for bad in (good.long(), good[:3], good.to("meta")):
-        with pytest.raises(ValueError):
-            sequence._slots(bad, 4, 7, "state", dev)
-
-
-def test_step_forms_refuse_gradients():
-    p = torch.zeros(3, requires_grad=True)
-    with pytest.raises(ValueError, match="no_grad"):
-        sequence._refuse_grad("step", None, p)
-    with torch.no_grad():
-        sequence._refuse_grad("step", None, p)
 
 
 # ---------------------------------------------------------------- the definitions
