@@ -16,10 +16,15 @@ int seq_cuda_fail(cudaError_t e);
 
 namespace seq {
 
-// out[i] = sum over c < chunks of part[c * stride + i] for i < m, in a fixed
-// order in fp32, rounded once to `dtype`.
-cudaError_t launch_reduce(const float* part, int chunks, long long stride, long long m, void* out, int dtype,
-                          cudaStream_t stream);
+// Sums of partial results: with p running over chunks, part[p * stride + i], i
+// counting through the outputs' elements one output after the other.  In a fixed
+// order, in fp32, rounded once to each output's type; outputs may be null.
+struct ReduceOut {
+  void* out;
+  long long m;  // elements
+  int dtype;
+};
+cudaError_t launch_reduce(const float* part, long long chunks, const ReduceOut (&outs)[3], cudaStream_t stream);
 
 // How the convolution's backward pass is cut (pt_seq_conv.cuh).
 struct ConvBwdPlan {

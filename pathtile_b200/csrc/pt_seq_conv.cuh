@@ -514,10 +514,8 @@ cudaError_t conv_bwd(const pt_conv_args& a, float* ws, int sm_count, cudaStream_
   });
   if (e != cudaSuccess) return e;
   const int out = a.param_f32 ? PT_F32 : a.dtype;
-  const long long m = static_cast<long long>(a.dim) * a.taps, all = m + a.dim;
-  if (a.dw && (e = launch_reduce(ws, p.chunks, all, m, a.dw, out, stream)) != cudaSuccess) return e;
-  if (a.dbias && (e = launch_reduce(ws + m, p.chunks, all, a.dim, a.dbias, out, stream)) != cudaSuccess) return e;
-  return cudaSuccess;
+  const long long m = static_cast<long long>(a.dim) * a.taps;
+  return launch_reduce(ws, p.chunks, {{a.dw, m, out}, {a.dbias, a.dim, out}, {nullptr, 0, out}}, stream);
 }
 
 template <class T>

@@ -21,11 +21,18 @@ namespace pt {
 namespace seq {
 namespace {
 
-constexpr int kNormMaxThreads = 1024;
+// What is fused: the common forms have kernels of their own (registers), any
+// other combination runs the general one.
+enum NormForm { kGated, kResidual, kAny };
 
-// V parameters from index i on.
+// V parameters from index i on (zeros from no pointer).
 template <class T, int V>
 __device__ __forceinline__ void load_param(const void* p, int i, int n, bool f32, float (&out)[V]) {
+  if (!p) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] = 0.f;
+    return;
+  }
   if (f32) {
     Pack<float, V> w;
     w.load(static_cast<const float*>(p) + i, n, true);
@@ -62,37 +69,53 @@ __device__ __forceinline__ float2 block_sum(float p, float q, float2 (*buf)[32],
   return make_float2(p, q);
 }
 
-template <class T, class R, int V, int NV>
-__global__ void __launch_bounds__(kNormMaxThreads) seq_norm_fwd_kernel(pt_norm_args a, int width, long long stride) {
+// One part of a row as it lies in memory.
+template <class T, class R, int V, int NV, int FORM>
+struct NormRow {
+  Pack<T, V> x[NV], gate[FORM == kResidual ? 1 : NV];
+  Pack<R, V> res[FORM == kGated ? 1 : NV];
+};
+
+template <class T, class R, int V, int NV, int FORM, int MAXT>
+__global__ void __launch_bounds__(MAXT) seq_norm_fwd_kernel(pt_norm_args a, int width, long long stride) {
   __shared__ float2 buf[2][32];
   const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
   const int c0 = static_cast<int>(blockIdx.x % a.groups) * width;
+  const bool gated = FORM == kGated || (FORM == kAny && a.gate);
+  const bool resid = FORM == kResidual || (FORM == kAny && a.residual);
+  const bool scaled = FORM != kGated && a.scale;
   float w[NV][V], sc[NV][V];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int i = (k * threads + tid) * V;
     if (i < width) {
       load_param<T, V>(a.weight, c0 + i, V, a.param_f32, w[k]);
-      if (a.scale) load_param<T, V>(a.scale, c0 + i, V, a.param_f32, sc[k]);
+      if (scaled) load_param<T, V>(a.scale, c0 + i, V, a.param_f32, sc[k]);
     }
   }
-  int slot = 0;
-  for (long long row = blockIdx.x / a.groups; row < a.rows; row += stride, slot ^= 1) {
-    const T* x = static_cast<const T*>(a.x) + row * a.x_row + c0;
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * a.gate_row + c0 : nullptr;
-    const R* res = a.residual ? static_cast<const R*>(a.residual) + row * a.residual_row + c0 : nullptr;
-    const long long o = row * a.dim + c0;
-    Pack<T, V> px[NV], pg[NV];
-    Pack<R, V> pr[NV];
+  NormRow<T, R, V, NV, FORM> next;
+  auto load = [&](long long row) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int i = (k * threads + tid) * V;
       if (i < width) {
-        px[k].load(x + i, V, true);
-        if (gate) pg[k].load(gate + i, V, true);
-        if (res) pr[k].load(res + i, V, true);
+        next.x[k].load(static_cast<const T*>(a.x) + row * a.x_row + c0 + i, V, true);
+        if constexpr (FORM != kResidual) {
+          if (gated) next.gate[k].load(static_cast<const T*>(a.gate) + row * a.gate_row + c0 + i, V, true);
+        }
+        if constexpr (FORM != kGated) {
+          if (resid) next.res[k].load(static_cast<const R*>(a.residual) + row * a.residual_row + c0 + i, V, true);
+        }
       }
     }
+  };
+  int slot = 0;
+  long long row = blockIdx.x / a.groups;
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += stride, slot ^= 1) {
+    NormRow<T, R, V, NV, FORM> in = next;
+    if (row + stride < a.rows) load(row + stride);  // on its way while this row is worked on
+    const long long o = row * a.dim + c0;
     float r[NV][V], ss = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -100,18 +123,24 @@ __global__ void __launch_bounds__(kNormMaxThreads) seq_norm_fwd_kernel(pt_norm_a
       if (i < width) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          float u = px[k].f(v);
-          if (gate) u *= siluf(pg[k].f(v));
-          if (a.scale) u *= sc[k][v];
-          if (res) {
-            // The stream that goes on is what is normalised: rounded to its type first.
-            pr[k].set(v, pr[k].f(v) + u);
-            u = pr[k].f(v);
+          float u = in.x[k].f(v);
+          if constexpr (FORM != kResidual) {
+            if (gated) u *= siluf(in.gate[k].f(v));
+          }
+          if (scaled) u *= sc[k][v];
+          if constexpr (FORM != kGated) {
+            if (resid) {
+              // The stream that goes on is what is normalised: rounded to its type first.
+              in.res[k].set(v, in.res[k].f(v) + u);
+              u = in.res[k].f(v);
+            }
           }
           r[k][v] = u;
           ss = fmaf(u, u, ss);
         }
-        if (res) pr[k].store(static_cast<R*>(a.r) + o + i, V, true);
+        if constexpr (FORM != kGated) {
+          if (resid) in.res[k].store(static_cast<R*>(a.r) + o + i, V, true);
+        }
       }
     }
     const float rstd = rsqrtf(block_sum(ss, 0.f, buf, slot).x / static_cast<float>(width) + a.eps);
@@ -128,59 +157,81 @@ __global__ void __launch_bounds__(kNormMaxThreads) seq_norm_fwd_kernel(pt_norm_a
   }
 }
 
-template <class T, class R, int V, int NV>
-__global__ void __launch_bounds__(kNormMaxThreads)
-    seq_norm_bwd_kernel(pt_norm_args a, float* part, int width, long long stride) {
+template <class T, class R, int V, int NV, int FORM>
+struct NormGradRow {
+  Pack<T, V> dy[NV], x[NV], gate[FORM == kResidual ? 1 : NV];
+  Pack<R, V> r[FORM == kGated ? 1 : NV], dr[FORM == kGated ? 1 : NV];
+};
+
+template <class T, class R, int V, int NV, int FORM, int MAXT>
+__global__ void __launch_bounds__(MAXT) seq_norm_bwd_kernel(pt_norm_args a, float* part, int width, long long stride) {
   __shared__ float2 buf[2][32];
   const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
   const int c0 = static_cast<int>(blockIdx.x % a.groups) * width;
-  const bool need_x = !a.residual || a.gate || (a.scale && a.dscale);
-  float dw[NV][V], ds[NV][V];
+  const bool gated = FORM == kGated || (FORM == kAny && a.gate);
+  const bool resid = FORM == kResidual || (FORM == kAny && a.residual);
+  const bool scaled = FORM != kGated && a.scale;
+  const bool need_x = !resid || gated || (scaled && a.dscale);
+  const bool more = FORM != kGated && a.dr;
+  float w[NV][V], sc[FORM == kGated ? 1 : NV][V], dw[NV][V], ds[FORM == kGated ? 1 : NV][V];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+  for (int k = 0; k < NV; ++k) {
+    const int i = (k * threads + tid) * V;
 #pragma unroll
-    for (int v = 0; v < V; ++v) dw[k][v] = ds[k][v] = 0.f;
-  int slot = 0;
-  for (long long row = blockIdx.x / a.groups; row < a.rows; row += stride, slot ^= 1) {
-    const long long o = row * a.dim + c0;
-    const T* x = static_cast<const T*>(a.x) + row * a.x_row + c0;
-    const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * a.gate_row + c0 : nullptr;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_row + c0;
-    const R* dr = a.dr ? static_cast<const R*>(a.dr) + row * a.dr_row + c0 : nullptr;
-    Pack<T, V> px[NV], pg[NV], py[NV];
-    Pack<R, V> pr[NV], pd[NV];
+    for (int v = 0; v < V; ++v) {
+      dw[k][v] = 0.f;
+      if constexpr (FORM != kGated) ds[k][v] = 0.f;
+    }
+    if (i < width) {
+      load_param<T, V>(a.weight, c0 + i, V, a.param_f32, w[k]);
+      if constexpr (FORM != kGated) {
+        if (scaled) load_param<T, V>(a.scale, c0 + i, V, a.param_f32, sc[k]);
+      }
+    }
+  }
+  NormGradRow<T, R, V, NV, FORM> next;
+  auto load = [&](long long row) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int i = (k * threads + tid) * V;
       if (i < width) {
-        py[k].load(dy + i, V, true);
-        if (need_x) px[k].load(x + i, V, true);
-        if (gate) pg[k].load(gate + i, V, true);
-        if (a.residual) pr[k].load(static_cast<const R*>(a.r) + o + i, V, true);
-        if (dr) pd[k].load(dr + i, V, true);
+        next.dy[k].load(static_cast<const T*>(a.dy) + row * a.dy_row + c0 + i, V, true);
+        if (need_x) next.x[k].load(static_cast<const T*>(a.x) + row * a.x_row + c0 + i, V, true);
+        if constexpr (FORM != kResidual) {
+          if (gated) next.gate[k].load(static_cast<const T*>(a.gate) + row * a.gate_row + c0 + i, V, true);
+        }
+        if constexpr (FORM != kGated) {
+          if (resid) next.r[k].load(static_cast<const R*>(a.r) + row * a.dim + c0 + i, V, true);
+          if (more) next.dr[k].load(static_cast<const R*>(a.dr) + row * a.dr_row + c0 + i, V, true);
+        }
       }
     }
+  };
+  int slot = 0;
+  long long row = blockIdx.x / a.groups;
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += stride, slot ^= 1) {
+    const NormGradRow<T, R, V, NV, FORM> in = next;
+    if (row + stride < a.rows) load(row + stride);  // on its way while this row is worked on
+    const long long o = row * a.dim + c0;
     float r[NV][V], ss = 0.f, sv = 0.f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int i = (k * threads + tid) * V;
       if (i < width) {
-        float w[V], sc[V];
-        load_param<T, V>(a.weight, c0 + i, V, a.param_f32, w);
-        if (a.scale && !a.residual) load_param<T, V>(a.scale, c0 + i, V, a.param_f32, sc);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           float u;
-          if (a.residual) {
-            u = pr[k].f(v);
+          if (resid) {
+            u = in.r[FORM == kGated ? 0 : k].f(v);
           } else {
-            u = px[k].f(v);
-            if (gate) u *= siluf(pg[k].f(v));
-            if (a.scale) u *= sc[v];
+            u = in.x[k].f(v);
+            if (gated) u *= siluf(in.gate[FORM == kResidual ? 0 : k].f(v));
+            if (scaled) u *= sc[FORM == kGated ? 0 : k][v];
           }
           r[k][v] = u;
           ss = fmaf(u, u, ss);
-          sv = fmaf(py[k].f(v) * w[v], u, sv);
+          sv = fmaf(in.dy[k].f(v) * w[k][v], u, sv);
         }
       }
     }
@@ -191,30 +242,39 @@ __global__ void __launch_bounds__(kNormMaxThreads)
     for (int k = 0; k < NV; ++k) {
       const int i = (k * threads + tid) * V;
       if (i < width) {
-        float w[V], sc[V];
-        load_param<T, V>(a.weight, c0 + i, V, a.param_f32, w);
-        if (a.scale) load_param<T, V>(a.scale, c0 + i, V, a.param_f32, sc);
         Pack<T, V> ox, og;
         Pack<R, V> ores;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float hat = r[k][v] * rstd, y = py[k].f(v);
+          const float hat = r[k][v] * rstd, y = in.dy[k].f(v);
           dw[k][v] = fmaf(y, hat, dw[k][v]);
-          float d = rstd * (y * w[v] - hat * mean);
-          if (dr) d += pd[k].f(v);
-          if (a.residual) ores.set(v, d);
+          float d = rstd * (y * w[k][v] - hat * mean);
+          if constexpr (FORM != kGated) {
+            if (more) d += in.dr[k].f(v);
+            if (resid) ores.set(v, d);
+          }
           float sig = 0.f, gv = 0.f, open = 1.f;
-          if (gate) gv = pg[k].f(v), sig = sigmoidf(gv), open = gv * sig;
-          if (a.scale) {
-            if (need_x) ds[k][v] = fmaf(d, px[k].f(v) * open, ds[k][v]);
-            d *= sc[v];
+          if constexpr (FORM != kResidual) {
+            if (gated) gv = in.gate[k].f(v), sig = sigmoidf(gv), open = gv * sig;
+          }
+          if constexpr (FORM != kGated) {
+            if (scaled) {
+              if (need_x) ds[k][v] = fmaf(d, in.x[k].f(v) * open, ds[k][v]);
+              d *= sc[k][v];
+            }
           }
           ox.set(v, d * open);
-          if (gate) og.set(v, d * px[k].f(v) * silu_grad(gv, sig));
+          if constexpr (FORM != kResidual) {
+            if (gated) og.set(v, d * in.x[k].f(v) * silu_grad(gv, sig));
+          }
         }
         if (a.dx) ox.store(static_cast<T*>(a.dx) + o + i, V, true);
-        if (a.dgate) og.store(static_cast<T*>(a.dgate) + o + i, V, true);
-        if (a.dresidual) ores.store(static_cast<R*>(a.dresidual) + o + i, V, true);
+        if constexpr (FORM != kResidual) {
+          if (a.dgate) og.store(static_cast<T*>(a.dgate) + o + i, V, true);
+        }
+        if constexpr (FORM != kGated) {
+          if (a.dresidual) ores.store(static_cast<R*>(a.dresidual) + o + i, V, true);
+        }
       }
     }
   }
@@ -226,19 +286,29 @@ __global__ void __launch_bounds__(kNormMaxThreads)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         mine[c0 + i + v] = dw[k][v];
-        if (a.dscale) mine[a.dim + c0 + i + v] = ds[k][v];
+        if constexpr (FORM != kGated) {
+          if (a.dscale) mine[a.dim + c0 + i + v] = ds[k][v];
+        }
       }
     }
   }
 }
 
+// Words per thread and the most threads of a block, which fix the registers
+// (64 Ki over the threads): rows of up to 512 words (single elements: 2048) and
+// twice that keep everything in registers, longer ones spill.
+template <int V, int NV, int MAXT>
+struct NormSize {
+  static constexpr int kV = V, kNV = NV, kMaxT = MAXT;
+};
+
 struct NormPlan {
   bool wide;
-  int nv, threads, blocks;  // blocks: per group of columns
+  int size, threads, blocks;  // size: 0, 1, 2 as above; blocks: per group of columns
 };
 
 template <class T, class R>
-NormPlan norm_plan(const pt_norm_args& a, int sm_count, bool backward) {
+NormPlan norm_size(const pt_norm_args& a) {
   constexpr int W = 16 / static_cast<int>(sizeof(T));
   const int width = a.dim / a.groups;
   auto ok = [&](const void* p, long long s) { return aligned(p, 16) && (!p || s % W == 0); };
@@ -247,36 +317,67 @@ NormPlan norm_plan(const pt_norm_args& a, int sm_count, bool backward) {
            ok(a.weight, 0) && ok(a.scale, 0) && ok(a.y, 0) && ok(a.r, 0) && ok(a.dy, a.dy_row) && ok(a.dr, a.dr_row) &&
            ok(a.dx, 0) && ok(a.dgate, 0) && ok(a.dresidual, 0);
   const int v = p.wide ? W : 1;
-  const int words = static_cast<int>(cdiv(width, v));
-  // One word per thread up to 1024 threads (single elements: four), more beyond.
-  if (p.wide)
-    p.nv = words <= 1024 ? 1 : words <= 2048 ? 2 : 8 / (W / 4);
-  else
-    p.nv = words <= 4096 ? 4 : 32;
-  p.threads = static_cast<int>(cdiv(cdiv(words, p.nv), 32)) * 32;
-  // Forward one wave of the SMs' 2048 threads, twice; backward one (each block writes a partial sum).
-  const long long want = cdiv(static_cast<long long>(sm_count) * (backward ? 1024 : 4096) / p.threads, a.groups);
-  p.blocks = static_cast<int>(a.rows < want ? a.rows : want);
+  const int words = static_cast<int>(cdiv(width, v)), one = p.wide ? 1 : 4;
+  p.size = words <= 512 * one ? 0 : words <= 1024 * one ? 1 : 2;
+  const int nv = p.size == 0 ? one : p.size == 1 ? 2 * one : p.wide ? PT_NORM_MAX_WIDTH / 1024 / W : 32;
+  p.threads = static_cast<int>(cdiv(cdiv(words, nv), 32)) * 32;
   return p;
 }
 
+// Calls fn(size, form) with both as constants.
 template <class T, class R, class F>
-cudaError_t by_plan(const NormPlan& p, F&& fn) {
+cudaError_t by_plan(const pt_norm_args& a, const NormPlan& p, F&& fn) {
   constexpr int W = 16 / static_cast<int>(sizeof(T));
-  if (p.wide) {
-    if (p.nv == 1) return fn(std::integral_constant<int, W>(), std::integral_constant<int, 1>());
-    if (p.nv == 2) return fn(std::integral_constant<int, W>(), std::integral_constant<int, 2>());
-    return fn(std::integral_constant<int, W>(), std::integral_constant<int, 8 / (W / 4)>());
+  auto sized = [&](auto form) -> cudaError_t {
+    if (p.wide) {
+      if (p.size == 0) return fn(NormSize<W, 1, 512>(), form);
+      if (p.size == 1) return fn(NormSize<W, 2, 512>(), form);
+    } else {
+      if (p.size == 0) return fn(NormSize<1, 4, 512>(), form);
+      if (p.size == 1) return fn(NormSize<1, 8, 512>(), form);
+    }
+    return cudaErrorInvalidValue;
+  };
+  if (p.size == 2) {
+    constexpr auto any = std::integral_constant<int, kAny>();
+    if (p.wide) return fn(NormSize<W, PT_NORM_MAX_WIDTH / 1024 / W, 1024>(), any);
+    return fn(NormSize<1, 32, 1024>(), any);
   }
-  if (p.nv == 4) return fn(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
-  return fn(std::integral_constant<int, 1>(), std::integral_constant<int, 32>());
+  if (a.gate && !a.residual && !a.scale) return sized(std::integral_constant<int, kGated>());
+  if (a.residual && !a.gate) return sized(std::integral_constant<int, kResidual>());
+  return sized(std::integral_constant<int, kAny>());
+}
+
+template <class T, class R, class Z, int FORM>
+const void* norm_kernel(bool backward) {
+  return backward ? reinterpret_cast<const void*>(&seq_norm_bwd_kernel<T, R, Z::kV, Z::kNV, FORM, Z::kMaxT>)
+                  : reinterpret_cast<const void*>(&seq_norm_fwd_kernel<T, R, Z::kV, Z::kNV, FORM, Z::kMaxT>);
+}
+
+// One wave: as many blocks as fit on the SMs, so that all walk about as many rows.
+template <class T, class R>
+cudaError_t norm_plan(const pt_norm_args& a, int sm_count, bool backward, NormPlan& p) {
+  p = norm_size<T, R>(a);
+  p.blocks = static_cast<int>(a.rows < sm_count ? a.rows : sm_count);
+  if (a.rows * a.groups <= sm_count) return cudaSuccess;
+  int per_sm = 1;
+  const cudaError_t e = by_plan<T, R>(a, p, [&](auto size, auto form) {
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+        &per_sm, norm_kernel<T, R, decltype(size), decltype(form)::value>(backward), p.threads, 0);
+  });
+  const long long want = cdiv(static_cast<long long>(sm_count) * (per_sm > 0 ? per_sm : 1), a.groups);
+  p.blocks = static_cast<int>(a.rows < want ? a.rows : want);
+  return e;
 }
 
 template <class T, class R>
 cudaError_t norm_fwd(const pt_norm_args& a, int sm_count, cudaStream_t stream) {
-  const NormPlan p = norm_plan<T, R>(a, sm_count, false);
-  return by_plan<T, R>(p, [&](auto vc, auto nc) {
-    seq_norm_fwd_kernel<T, R, decltype(vc)::value, decltype(nc)::value>
+  NormPlan p;
+  cudaError_t e = norm_plan<T, R>(a, sm_count, false, p);
+  if (e != cudaSuccess) return e;
+  return by_plan<T, R>(a, p, [&](auto size, auto form) {
+    using Z = decltype(size);
+    seq_norm_fwd_kernel<T, R, Z::kV, Z::kNV, decltype(form)::value, Z::kMaxT>
         <<<static_cast<unsigned>(p.blocks * a.groups), p.threads, 0, stream>>>(a, a.dim / a.groups, p.blocks);
     return cudaGetLastError();
   });
@@ -284,17 +385,18 @@ cudaError_t norm_fwd(const pt_norm_args& a, int sm_count, cudaStream_t stream) {
 
 template <class T, class R>
 cudaError_t norm_bwd(const pt_norm_args& a, float* ws, int sm_count, cudaStream_t stream) {
-  const NormPlan p = norm_plan<T, R>(a, sm_count, true);
-  cudaError_t e = by_plan<T, R>(p, [&](auto vc, auto nc) {
-    seq_norm_bwd_kernel<T, R, decltype(vc)::value, decltype(nc)::value>
+  NormPlan p;
+  cudaError_t e = norm_plan<T, R>(a, sm_count, true, p);
+  if (e != cudaSuccess) return e;
+  e = by_plan<T, R>(a, p, [&](auto size, auto form) {
+    using Z = decltype(size);
+    seq_norm_bwd_kernel<T, R, Z::kV, Z::kNV, decltype(form)::value, Z::kMaxT>
         <<<static_cast<unsigned>(p.blocks * a.groups), p.threads, 0, stream>>>(a, ws, a.dim / a.groups, p.blocks);
     return cudaGetLastError();
   });
   if (e != cudaSuccess) return e;
   const int out = a.param_f32 ? PT_F32 : a.dtype;
-  if (a.dweight && (e = launch_reduce(ws, p.blocks, 2LL * a.dim, a.dim, a.dweight, out, stream)) != cudaSuccess) return e;
-  if (a.dscale) return launch_reduce(ws + a.dim, p.blocks, 2LL * a.dim, a.dim, a.dscale, out, stream);
-  return cudaSuccess;
+  return launch_reduce(ws, p.blocks, {{a.dweight, a.dim, out}, {a.dscale, a.dim, out}, {nullptr, 0, out}}, stream);
 }
 
 // Calls fn(T(), R()): R, the residual's type, is T or float.
@@ -306,16 +408,21 @@ cudaError_t by_types(const pt_norm_args& a, F&& fn) {
   });
 }
 
+struct ReduceArgs {
+  ReduceOut out[3];
+  long long end[3];  // first element behind each output
+};
+
 // One block: 32 columns x 8 threads that each add every eighth chunk.
-template <class O>
-__global__ void __launch_bounds__(256)
-    seq_reduce_kernel(const float* part, int chunks, long long stride, long long m, O* out) {
+__global__ void __launch_bounds__(256) seq_reduce_kernel(const float* part, long long chunks, ReduceArgs a) {
   __shared__ float buf[8][32];
   const int tx = static_cast<int>(threadIdx.x), ty = static_cast<int>(threadIdx.y);
-  const long long i = static_cast<long long>(blockIdx.x) * 32 + tx;
+  const long long i = static_cast<long long>(blockIdx.x) * 32 + tx, stride = a.end[2];
+  const int k = i < a.end[0] ? 0 : i < a.end[1] ? 1 : 2;
+  const bool in = i < stride && a.out[k].out;
   float s = 0.f;
-  if (i < m) {
-    int c = ty;
+  if (in) {
+    long long c = ty;
     for (; c + 24 < chunks; c += 32) {
       const float* p = part + c * stride + i;
       const float v0 = p[0], v1 = p[8 * stride], v2 = p[16 * stride], v3 = p[24 * stride];
@@ -325,23 +432,33 @@ __global__ void __launch_bounds__(256)
   }
   buf[ty][tx] = s;
   __syncthreads();
-  if (ty == 0 && i < m) {
+  if (ty == 0 && in) {
 #pragma unroll
     for (int r = 1; r < 8; ++r) s += buf[r][tx];
-    out[i] = from_f<O>(s);
+    const long long j = k ? i - a.end[k - 1] : i;
+    if (a.out[k].dtype == PT_F32)
+      static_cast<float*>(a.out[k].out)[j] = s;
+    else if (a.out[k].dtype == PT_BF16)
+      static_cast<__nv_bfloat16*>(a.out[k].out)[j] = from_f<__nv_bfloat16>(s);
+    else
+      static_cast<__half*>(a.out[k].out)[j] = from_f<__half>(s);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_reduce(const float* part, int chunks, long long stride, long long m, void* out, int dtype,
-                          cudaStream_t stream) {
-  return by_type(dtype, [&](auto t) {
-    using O = decltype(t);
-    seq_reduce_kernel<O><<<static_cast<unsigned>(cdiv(m, 32)), dim3(32, 8), 0, stream>>>(part, chunks, stride, m,
-                                                                                         static_cast<O*>(out));
-    return cudaGetLastError();
-  });
+cudaError_t launch_reduce(const float* part, long long chunks, const ReduceOut (&outs)[3], cudaStream_t stream) {
+  ReduceArgs a;
+  long long end = 0;
+  bool any = false;
+  for (int k = 0; k < 3; ++k) {
+    a.out[k] = outs[k];
+    a.end[k] = end += outs[k].m;
+    any |= outs[k].out && outs[k].m > 0;
+  }
+  if (!any) return cudaSuccess;
+  seq_reduce_kernel<<<static_cast<unsigned>(cdiv(end, 32)), dim3(32, 8), 0, stream>>>(part, chunks, a);
+  return cudaGetLastError();
 }
 
 cudaError_t launch_norm_fwd(const pt_norm_args& a, int sm_count, cudaStream_t stream) {
@@ -351,12 +468,9 @@ cudaError_t launch_norm_bwd(const pt_norm_args& a, float* ws, int sm_count, cuda
   return by_types(a, [&](auto t, auto r) { return norm_bwd<decltype(t), decltype(r)>(a, ws, sm_count, stream); });
 }
 size_t norm_bwd_workspace(const pt_norm_args& a, int sm_count) {
-  size_t n = 0;
-  by_types(a, [&](auto t, auto r) {
-    n = sizeof(float) * 2 * a.dim * static_cast<size_t>(norm_plan<decltype(t), decltype(r)>(a, sm_count, true).blocks);
-    return cudaSuccess;
-  });
-  return n;
+  NormPlan p;
+  const cudaError_t e = by_types(a, [&](auto t, auto r) { return norm_plan<decltype(t), decltype(r)>(a, sm_count, true, p); });
+  return e == cudaSuccess ? sizeof(float) * 2 * a.dim * static_cast<size_t>(p.blocks) : 0;
 }
 
 }  // namespace seq

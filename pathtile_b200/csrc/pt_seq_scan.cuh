@@ -544,7 +544,7 @@ struct BackwardSmem {
 template <class T, int S, bool PAD>
 __global__ void __launch_bounds__(kBlock, 2)
     seq_scan_bwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d, float* part_bc,
-                        float* part_a, float* part_d) {
+                        float* part_p) {
   using P = ScanShape<S>;
   extern __shared__ __align__(16) unsigned char smem[];
   auto& sm = *reinterpret_cast<BackwardSmem<S>*>(smem);
@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(kBlock, 2)
   const int tiles = max(0, (t1 - t0 + kTile - 1) / kTile);
   const long long ckpt_row = (static_cast<long long>(a.len) + kTile - 1) / kTile;
   const long long all = static_cast<long long>(a.dim) * a.state;
-  const long long piece = static_cast<long long>(chunk) * dm.segs + seg;
+  // This block's partial sums of dA [dim, state], dD [dim], ddt_bias [dim].
+  float* mine = part_p + (static_cast<long long>(chunk) * dm.segs + seg) * (all + 2 * a.dim);
   const int tid = static_cast<int>(threadIdx.x);
   // Tiles are taken from the last to the first; k counts them in that order.
   auto tile_of = [&](int k) { return t0 + (tiles - 1 - k) * kTile; };
@@ -668,8 +669,8 @@ __global__ void __launch_bounds__(kBlock, 2)
       float sD = 0.f, sb = 0.f;
 #pragma unroll
       for (int q = 0; q < kTile; ++q) sD += sm.accD[q][c], sb += sm.accb[q][c];
-      part_d[piece * 2 * a.dim + at.c0 + c] = sD;
-      part_d[piece * 2 * a.dim + a.dim + at.c0 + c] = sb;
+      mine[all + at.c0 + c] = sD;
+      mine[all + a.dim + at.c0 + c] = sb;
     }
     return;
   }
@@ -817,14 +818,14 @@ __global__ void __launch_bounds__(kBlock, 2)
     if (a.dh0 && seg == 0) store_states(a.dh0 + b * all, a, me, g);
     meet();  // the next row's tiles overwrite what this row's last gradients are made from
   }
-  if (part_a) {
+  if (a.dA) {
     Quad dA;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const float4 s = sm.accA[c][tid];
       dA[c][0] = pack2(s.x, s.y), dA[c][1] = pack2(s.z, s.w);
     }
-    store_states(part_a + piece * all, a, me, dA);
+    store_states(mine, a, me, dA);
   }
   meet();
 }
@@ -978,8 +979,7 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
     float* seg_h = ws;
     float* seg_d = ws + static_cast<size_t>(a.batch) * p.segs * a.dim * a.state;
     float* part_bc = ws + segment_floats(a, p);
-    float* part_a = part_bc + p.cblocks * rows * 8 * S;
-    float* part_d = part_a + pieces * all;
+    float* part_p = part_bc + p.cblocks * rows * 8 * S;
     const long long blocks = static_cast<long long>(p.cblocks) * a.groups;
     if (blocks * a.batch * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     cudaError_t e;
@@ -990,7 +990,7 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
     }
     auto kernel = a.state == 4 * S ? seq_scan_bwd_kernel<T, S, false> : seq_scan_bwd_kernel<T, S, true>;
     e = launch_with<BackwardSmem<S>>(kernel, blocks * pieces, kBlock, stream, a, dm, seg_h, seg_d,
-                                        a.dB || a.dC ? part_bc : nullptr, a.dA ? part_a : nullptr, part_d);
+                                        a.dB || a.dC ? part_bc : nullptr, part_p);
     if (e != cudaSuccess) return e;
     if (a.dB || a.dC) {
       const long long n = rows * 8 * S;
@@ -1000,13 +1000,8 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
       }
     }
-    const int n = static_cast<int>(pieces);
-    if (a.dA && (e = launch_reduce(part_a, n, all, all, a.dA, PT_F32, stream)) != cudaSuccess) return e;
-    if (a.dD && (e = launch_reduce(part_d, n, 2LL * a.dim, a.dim, a.dD, PT_F32, stream)) != cudaSuccess) return e;
-    if (a.ddt_bias &&
-        (e = launch_reduce(part_d + a.dim, n, 2LL * a.dim, a.dim, a.ddt_bias, PT_F32, stream)) != cudaSuccess)
-      return e;
-    return cudaSuccess;
+    return launch_reduce(part_p, pieces, {{a.dA, all, PT_F32}, {a.dD, a.dim, PT_F32}, {a.ddt_bias, a.dim, PT_F32}},
+                         stream);
   });
 }
 
