@@ -185,9 +185,12 @@ __device__ __forceinline__ void put_floats(float* dst, const float (&v)[E]) {
 #pragma unroll
     for (int i = 0; i < E / 4; ++i)
       reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else {
+  } else if constexpr (E % 2 == 0) {
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) reinterpret_cast<float2*>(dst)[i] = make_float2(v[2 * i], v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) dst[i] = v[i];
   }
 }
 template <int E>
@@ -198,12 +201,15 @@ __device__ __forceinline__ void get_floats(const float* src, float (&v)[E]) {
       const float4 f = reinterpret_cast<const float4*>(src)[i];
       v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
     }
-  } else {
+  } else if constexpr (E % 2 == 0) {
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
       const float2 f = reinterpret_cast<const float2*>(src)[i];
       v[2 * i] = f.x, v[2 * i + 1] = f.y;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = src[i];
   }
 }
 

@@ -38,21 +38,35 @@ namespace seq {
 constexpr int kTile = 16;  // steps per tile, and between checkpoints
 constexpr int kSub = 4;    // backward: steps whose states and decays are in registers together
 
-// A block: 4 warps that scan, 4 warps that stage.
-constexpr int kScanners = 128, kStagers = 128, kBlock = kScanners + kStagers;
+// A block: 4 warps that scan, 8 warps that stage.  Two blocks per SM are launched
+// with 80 registers for each thread; the stagers give up what the scanners need.
+// (Scanning alone takes 188 us and 640 us backward for 8 x 2048 x 2048 channels
+// with 16 states; with 4 staging warps the staging alone took 216 and 636 us.)
+constexpr int kScanners = 128, kStagers = 256, kBlock = kScanners + kStagers;
 constexpr int kScanWarps = kScanners / 32;
-// Backward, registers per thread: two blocks per SM are launched with 128 for
-// each thread; the scanners take 40 of the stagers'.
-constexpr int kScannerRegs = 168, kStagerRegs = 88;
+constexpr int kLaunchRegs = 80;
+constexpr int kFwdScannerRegs = 112, kFwdStagerRegs = 64;
+constexpr int kBwdScannerRegs = 144, kBwdStagerRegs = 48;
+static_assert(kScanners * kFwdScannerRegs + kStagers * kFwdStagerRegs <= kBlock * kLaunchRegs, "registers forward");
+static_assert(kScanners * kBwdScannerRegs + kStagers * kBwdStagerRegs <= kBlock * kLaunchRegs, "registers backward");
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 template <int S>
 struct ScanShape {
   static constexpr int kStates = 4 * S;                     // padded number of states
   static constexpr int kWarpCh = 2 * (32 / S);              // channels per scanning warp
   static constexpr int kCh = kScanWarps * kWarpCh;          // channels per block
-  static constexpr int kRowThreads = kStagers / kTile;      // threads that stage one step: 8
-  static constexpr int kE = kCh / kRowThreads;              // neighbouring channels a thread stages: 16, 8, 4, 2
-  static constexpr int kN = kStates / kRowThreads;          // states a thread stages
+  static constexpr int kRowThreads = kStagers / kTile;      // threads that stage one step: 16
+  static constexpr int kE = kCh / kRowThreads;              // neighbouring channels a thread stages: 8, 4, 2, 1
+  static constexpr int kN = (kStates + kRowThreads - 1) / kRowThreads;  // states a thread stages
 };
 
 // The whole block meets; scanners and stagers call it from their own code.
@@ -108,7 +122,10 @@ struct StateRow {
   }
   __device__ __forceinline__ void store(float* dst, int k) const {
 #pragma unroll
-    for (int i = 0; i < P::kN; ++i) dst[k + i * P::kRowThreads] = to_f<T>(v[i]);
+    for (int i = 0; i < P::kN; ++i) {
+      const int j = k + i * P::kRowThreads;
+      if (P::kStates % P::kRowThreads == 0 || j < P::kStates) dst[j] = to_f<T>(v[i]);
+    }
   }
 };
 
@@ -167,6 +184,7 @@ __device__ __forceinline__ void load_rates(const pt_scan_args& a, const Scanner<
 // A channel pair's values of one step, each twice: ready for packed arithmetic over states.
 struct Both {
   F2 v[2];
+  __device__ __forceinline__ Both() {}
   __device__ __forceinline__ explicit Both(const float* p) {
     const float2 f = *reinterpret_cast<const float2*>(p);
     v[0] = pack2(f.x, f.x), v[1] = pack2(f.y, f.y);
@@ -175,6 +193,7 @@ struct Both {
 // Four states' values of one step, in packed pairs.
 struct Four {
   F2 v[2];
+  __device__ __forceinline__ Four() {}
   __device__ __forceinline__ explicit Four(const float* p) {
     const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(p);
     v[0] = f.x, v[1] = f.y;
@@ -261,6 +280,7 @@ __global__ void __launch_bounds__(kBlock, 2)
   auto tile_of = [&](int k) { return t0 + (REV ? tiles - 1 - k : k) * kTile; };
   const int tid = static_cast<int>(threadIdx.x);
   if (tid >= kScanners) {
+    fewer_registers<kFwdStagerRegs>();
     const Stager<S> me(tid - kScanners, at.c0, at.nch);
     float bias[P::kE];
     me.params(a.dt_bias, bias);
@@ -310,6 +330,7 @@ __global__ void __launch_bounds__(kBlock, 2)
     }
     return;
   }
+  more_registers<kFwdScannerRegs>();
   const Scanner<S> me(tid, at.c0, at.nch);
   Quad A2, h = {};
   float dsum[2] = {0.f, 0.f};
@@ -379,6 +400,7 @@ __global__ void __launch_bounds__(kBlock, 2)
   const int tiles = max(0, (t1 - t0 + kTile - 1) / kTile);
   const int tid = static_cast<int>(threadIdx.x);
   if (tid >= kScanners) {
+    fewer_registers<kFwdStagerRegs>();
     const Stager<S> me(tid - kScanners, at.c0, at.nch);
     float bias[P::kE], Dv[P::kE];
     me.params(a.dt_bias, bias);
@@ -450,6 +472,7 @@ __global__ void __launch_bounds__(kBlock, 2)
     if (tiles > 0) finish(tiles - 1, x[0], z[0]);
     return;
   }
+  more_registers<kFwdScannerRegs>();
   const Scanner<S> me(tid, at.c0, at.nch);
   Quad A2, h = {};
   load_rates(a, me, A2);
@@ -461,29 +484,72 @@ __global__ void __launch_bounds__(kBlock, 2)
     const int st = k & 1;
     if (a.checkpoints)
       store_states(a.checkpoints + (b * ckpt_row + t0 / kTile + k) * a.dim * a.state, a, me, h);
-#pragma unroll 4
-    for (int i = 0; i < kTile; i += 2) {
-      float y[2][2];
+    {
+      // Decays of the next pair of steps are computed while this pair is scanned, and its sums cross the lanes one
+      // pair later: no instruction waits for the one before it.
+      F2 e[2][2][2];
+      Four Bn[2] = {Four(&sm.B[st][0][me.s0]), Four(&sm.B[st][1][me.s0])};
+      Both vn[2] = {Both(&sm.v[st][0][me.cl]), Both(&sm.v[st][1][me.cl])};
+      Both dn[2] = {Both(&sm.d[st][0][me.cl]), Both(&sm.d[st][1][me.cl])};
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const Both d(&sm.d[st][i + q][me.cl]), v(&sm.v[st][i + q][me.cl]);
-        const Four B(&sm.B[st][i + q][me.s0]), C(&sm.C[st][i + q][me.s0]);
+      for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int p = 0; p < 2; ++p)
-            h[c][p] = fma2(ex2x2(mul2(d.v[c], A2[c][p])), h[c][p], mul2(v.v[c], B.v[p]));
-          if constexpr (PAD) {
-            y[q][c] = dot2(h[c][1], C.v[1], dot2(h[c][0], C.v[0], 0.f, me.s0, a.state), me.s0 + 2, a.state);
-          } else {
-            const F2 s = fma2(h[c][1], C.v[1], mul2(h[c][0], C.v[0]));
-            y[q][c] = lo2(s) + hi2(s);
+          for (int p = 0; p < 2; ++p) e[q][c][p] = ex2x2(mul2(dn[q].v[c], A2[c][p]));
+      dn[0] = Both(&sm.d[st][2][me.cl]), dn[1] = Both(&sm.d[st][3][me.cl]);
+      float last[2][2];
+#pragma unroll
+      for (int i = 0; i < kTile; i += 2) {
+        F2 en[2][2][2];
+        Both v[2] = {vn[0], vn[1]};
+        Four B[2] = {Bn[0], Bn[1]};
+        const Four C[2] = {Four(&sm.C[st][i][me.s0]), Four(&sm.C[st][i + 1][me.s0])};
+        if (i + 2 < kTile) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int p = 0; p < 2; ++p) en[q][c][p] = ex2x2(mul2(dn[q].v[c], A2[c][p]));
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            vn[q] = Both(&sm.v[st][i + 2 + q][me.cl]);
+            Bn[q] = Four(&sm.B[st][i + 2 + q][me.s0]);
+            if (i + 4 < kTile) dn[q] = Both(&sm.d[st][i + 4 + q][me.cl]);
           }
         }
+        float y[2][2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) h[c][p] = fma2(e[q][c][p], h[c][p], mul2(v[q].v[c], B[q].v[p]));
+            if constexpr (PAD) {
+              y[q][c] = dot2(h[c][1], C[q].v[1], dot2(h[c][0], C[q].v[0], 0.f, me.s0, a.state), me.s0 + 2, a.state);
+            } else {
+              const F2 s = fma2(h[c][1], C[q].v[1], mul2(h[c][0], C[q].v[0]));
+              y[q][c] = lo2(s) + hi2(s);
+            }
+          }
+        if (i > 0) {
+          float first, second;
+          sum_slices<S>(last, me.slice, first, second);
+          put_sums<S>(sm.y[st], i - 2, me.cl, me.slice, first, second);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            last[q][c] = y[q][c];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) e[q][c][p] = en[q][c][p];
+          }
       }
       float first, second;
-      sum_slices<S>(y, me.slice, first, second);
-      put_sums<S>(sm.y[st], i, me.cl, me.slice, first, second);
+      sum_slices<S>(last, me.slice, first, second);
+      put_sums<S>(sm.y[st], kTile - 2, me.cl, me.slice, first, second);
     }
     meet();
   }
@@ -561,7 +627,7 @@ __global__ void __launch_bounds__(kBlock, 2)
   auto tile_of = [&](int k) { return t0 + (tiles - 1 - k) * kTile; };
 
   if (tid >= kScanners) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kStagerRegs));
+    fewer_registers<kBwdStagerRegs>();
     const Stager<S> me(tid - kScanners, at.c0, at.nch);
     float accD[P::kE] = {}, accb[P::kE] = {};
     for (int b = chunk; b < a.batch; b += dm.row_chunks) {
@@ -675,7 +741,7 @@ __global__ void __launch_bounds__(kBlock, 2)
     return;
   }
 
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kScannerRegs));
+  more_registers<kBwdScannerRegs>();
   const Scanner<S> me(tid, at.c0, at.nch);
   Quad A2;
   load_rates(a, me, A2);
@@ -941,6 +1007,11 @@ inline size_t segment_floats(const pt_scan_args& a, const ScanPlan& p) {
 template <class Smem, class K, class... A>
 cudaError_t launch_with(K kernel, long long grid, int threads, cudaStream_t stream, A... args) {
   constexpr int bytes = static_cast<int>(sizeof(Smem));
+  // The scanners wait for the registers that the split promises them: without those, no launch.
+  cudaFuncAttributes attr;
+  const cudaError_t known = cudaFuncGetAttributes(&attr, kernel);
+  if (known != cudaSuccess) return known;
+  if (attr.numRegs < kLaunchRegs) return cudaErrorLaunchOutOfResources;
   if (bytes > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
