@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "pathtile_b200.h"
 
@@ -31,6 +32,34 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// Two floats in a 64-bit register pair, for the packed fp32 instructions.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float lo2(F2 v) {
+  return __uint_as_float(static_cast<unsigned>(v));
+}
+__device__ __forceinline__ float hi2(F2 v) {
+  return __uint_as_float(static_cast<unsigned>(v >> 32));
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // E consecutive elements as they lie in memory: moved in words of up to 16 bytes.
 template <class T, int E>
 struct Pack {
@@ -87,6 +116,32 @@ struct Pack {
   }
   __device__ __forceinline__ float f(int i) const { return to_f<T>(v[i]); }
   __device__ __forceinline__ void set(int i, float x) { v[i] = from_f<T>(x); }
+  // Elements 2 i and 2 i + 1 (of a single element: itself and 0).
+  __device__ __forceinline__ F2 pair(int i) const {
+    if constexpr (E == 1) {
+      return pack2(to_f<T>(v[0]), 0.f);
+    } else if constexpr (sizeof(T) == 4) {
+      return pack2(v[2 * i], v[2 * i + 1]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const unsigned w = reinterpret_cast<const unsigned*>(v)[i];
+      return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    } else {
+      const float2 w = __half22float2(reinterpret_cast<const __half2*>(v)[i]);
+      return pack2(w.x, w.y);
+    }
+  }
+  __device__ __forceinline__ void set_pair(int i, F2 x) {
+    if constexpr (E == 1) {
+      v[0] = from_f<T>(lo2(x));
+    } else if constexpr (sizeof(T) == 4) {
+      v[2 * i] = lo2(x), v[2 * i + 1] = hi2(x);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      reinterpret_cast<__nv_bfloat162*>(v)[i] = __floats2bfloat162_rn(lo2(x), hi2(x));
+    } else {
+      reinterpret_cast<__half2*>(v)[i] = __floats2half2_rn(lo2(x), hi2(x));
+    }
+  }
+  static constexpr int kPairs = (E + 1) / 2;
 };
 
 // A parameter in fp32 or in the activations' type.
@@ -116,52 +171,35 @@ __device__ __forceinline__ float siluf(float v) { return v * sigmoidf(v); }
 // d silu(v) / dv, with s = sigmoid(v).
 __device__ __forceinline__ float silu_grad(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
 
+__device__ __forceinline__ F2 ex2x2(F2 x) { return pack2(ex2(lo2(x)), ex2(hi2(x))); }
+__device__ __forceinline__ F2 same2(float v) { return pack2(v, v); }
+__device__ __forceinline__ F2 rcp2(F2 v) { return pack2(rcp(lo2(v)), rcp(hi2(v))); }
+__device__ __forceinline__ F2 sigmoid2(F2 v) {
+  return rcp2(add2(ex2x2(mul2(v, same2(-kLog2e))), same2(1.f)));
+}
+// d silu(v) / dv, with s = sigmoid(v): s (1 + v (1 - s)).
+__device__ __forceinline__ F2 silu_grad2(F2 v, F2 s) {
+  return mul2(s, fma2(v, fma2(s, same2(-1.f), same2(1.f)), same2(1.f)));
+}
+
 // log(1 + e^v).  With e = e^-|v| <= 1 it is max(v, 0) + log(1 + e), and
 // log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: the odd series up to s^13
 // leaves s^14 / 15 < 2e-8 of the value, so small results keep their relative
 // precision (log(1 + e) computed as such would not).
-__device__ __forceinline__ float softplusf(float v) {
-  const float e = ex2(-fabsf(v) * kLog2e);
-  const float s = e * rcp(2.f + e), q = s * s;
-  float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-  p = fmaf(p, q, 1.f / 9.f);
-  p = fmaf(p, q, 1.f / 7.f);
-  p = fmaf(p, q, 1.f / 5.f);
-  p = fmaf(p, q, 1.f / 3.f);
-  p = fmaf(p, q, 1.f);
+__device__ __forceinline__ F2 softplus2(F2 v) {
+  const F2 m = mul2(v, same2(kLog2e));
+  const F2 e = pack2(ex2(-fabsf(lo2(m))), ex2(-fabsf(hi2(m))));
+  const F2 s = mul2(e, rcp2(add2(e, same2(2.f)))), q = mul2(s, s);
+  F2 p = fma2(q, same2(1.f / 13.f), same2(1.f / 11.f));
+  p = fma2(p, q, same2(1.f / 9.f));
+  p = fma2(p, q, same2(1.f / 7.f));
+  p = fma2(p, q, same2(1.f / 5.f));
+  p = fma2(p, q, same2(1.f / 3.f));
+  p = fma2(p, q, same2(1.f));
   // A NaN stays one: fmaxf would drop it, e carries it.
-  return fmaf(s + s, p, fmaxf(v, 0.f));
+  return fma2(add2(s, s), p, pack2(fmaxf(lo2(v), 0.f), fmaxf(hi2(v), 0.f)));
 }
-
-// Two floats in a 64-bit register pair, for the packed fp32 instructions.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 pack2(float a, float b) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float lo2(F2 v) {
-  return __uint_as_float(static_cast<unsigned>(v));
-}
-__device__ __forceinline__ float hi2(F2 v) {
-  return __uint_as_float(static_cast<unsigned>(v >> 32));
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 ex2x2(F2 x) { return pack2(ex2(lo2(x)), ex2(hi2(x))); }
+__device__ __forceinline__ float softplusf(float v) { return lo2(softplus2(same2(v))); }
 
 // Copies of 4, 8 or 16 bytes from global to shared memory that run on while the thread works.
 template <int BYTES>
@@ -178,38 +216,30 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// E floats of shared memory (16-byte aligned where E is 4 or more).
+// E floats of shared memory in packed pairs (16-byte aligned where E is 4 or more).
 template <int E>
-__device__ __forceinline__ void put_floats(float* dst, const float (&v)[E]) {
-  if constexpr (E % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i)
-      reinterpret_cast<float4*>(dst)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else if constexpr (E % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) reinterpret_cast<float2*>(dst)[i] = make_float2(v[2 * i], v[2 * i + 1]);
+__device__ __forceinline__ void put_pairs(float* dst, const F2 (&v)[(E + 1) / 2]) {
+  if constexpr (E == 1) {
+    *dst = lo2(v[0]);
+  } else if constexpr (E == 2) {
+    *reinterpret_cast<F2*>(dst) = v[0];
   } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) dst[i] = v[i];
+    for (int i = 0; i < E / 4; ++i) reinterpret_cast<ulonglong2*>(dst)[i] = make_ulonglong2(v[2 * i], v[2 * i + 1]);
   }
 }
 template <int E>
-__device__ __forceinline__ void get_floats(const float* src, float (&v)[E]) {
-  if constexpr (E % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < E / 4; ++i) {
-      const float4 f = reinterpret_cast<const float4*>(src)[i];
-      v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
-    }
-  } else if constexpr (E % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const float2 f = reinterpret_cast<const float2*>(src)[i];
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
-    }
+__device__ __forceinline__ void get_pairs(const float* src, F2 (&v)[(E + 1) / 2]) {
+  if constexpr (E == 1) {
+    v[0] = pack2(*src, 0.f);
+  } else if constexpr (E == 2) {
+    v[0] = *reinterpret_cast<const F2*>(src);
   } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = src[i];
+    for (int i = 0; i < E / 4; ++i) {
+      const ulonglong2 f = reinterpret_cast<const ulonglong2*>(src)[i];
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
   }
 }
 

@@ -56,12 +56,12 @@ struct Packed {
   template <class T>
   __device__ __forceinline__ void from(const Pack<T, V>& a) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = pack2(a.f(2 * i), 2 * i + 1 < V ? a.f(2 * i + 1 < V ? 2 * i + 1 : 0) : 0.f);
+    for (int i = 0; i < N; ++i) p[i] = a.pair(i);
   }
   template <class T>
   __device__ __forceinline__ void to(Pack<T, V>& a) const {
 #pragma unroll
-    for (int v = 0; v < V; ++v) a.set(v, v & 1 ? hi2(p[v / 2]) : lo2(p[v / 2]));
+    for (int i = 0; i < N; ++i) a.set_pair(i, p[i]);
   }
 };
 
@@ -124,12 +124,6 @@ __device__ __forceinline__ void load_taps(const pt_conv_args& a, int c0, float* 
     const float b1 = in && a.bias && v1 > v0 ? param<T>(a.bias, c0 + me * V + v1, a.param_f32) : 0.f;
     taps.bias.p[i] = pack2(b0, b1);
   }
-}
-
-__device__ __forceinline__ F2 sigmoid2(F2 v) {
-  const F2 m = mul2(v, pack2(-kLog2e, -kLog2e));
-  const F2 d = add2(pack2(ex2(lo2(m)), ex2(hi2(m))), pack2(1.f, 1.f));
-  return pack2(rcp(lo2(d)), rcp(hi2(d)));
 }
 
 template <class T, int K, int V>
@@ -256,10 +250,8 @@ __device__ __forceinline__ void conv_bwd_stretch(const pt_conv_args& a, const Ta
 #pragma unroll
       for (int i = 0; i < Packed<V>::N; ++i) {
         if (a.silu) {
-          const F2 one = pack2(1.f, 1.f), pre = taps.pre(win, i), sig = sigmoid2(pre);
-          // act' = sig (1 + pre (1 - sig))
-          const F2 rest = fma2(sig, pack2(-1.f, -1.f), one);
-          g.p[i] = mul2(g.p[i], mul2(sig, fma2(pre, rest, one)));
+          const F2 pre = taps.pre(win, i), sig = sigmoid2(pre);
+          g.p[i] = mul2(g.p[i], silu_grad2(pre, sig));
         }
         // Steps behind the row's end have no output; their window may hold anything.
         if (t >= len) g.p[i] = 0;

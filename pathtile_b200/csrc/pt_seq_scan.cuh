@@ -38,17 +38,23 @@ namespace seq {
 constexpr int kTile = 16;  // steps per tile, and between checkpoints
 constexpr int kSub = 4;    // backward: steps whose states and decays are in registers together
 
-// A block: 4 warps that scan, 8 warps that stage.  Two blocks per SM are launched
-// with 80 registers for each thread; the stagers give up what the scanners need.
-// (Scanning alone takes 188 us and 640 us backward for 8 x 2048 x 2048 channels
-// with 16 states; with 4 staging warps the staging alone took 216 and 636 us.)
-constexpr int kScanners = 128, kStagers = 256, kBlock = kScanners + kStagers;
-constexpr int kScanWarps = kScanners / 32;
-constexpr int kLaunchRegs = 80;
-constexpr int kFwdScannerRegs = 112, kFwdStagerRegs = 64;
-constexpr int kBwdScannerRegs = 144, kBwdStagerRegs = 48;
-static_assert(kScanners * kFwdScannerRegs + kStagers * kFwdStagerRegs <= kBlock * kLaunchRegs, "registers forward");
-static_assert(kScanners * kBwdScannerRegs + kStagers * kBwdStagerRegs <= kBlock * kLaunchRegs, "registers backward");
+// A block: 4 warps that scan, and some that stage.  Two blocks per SM are launched
+// with the registers that leaves for each thread; the stagers give up what the
+// scanners need.
+constexpr int kScanners = 128, kScanWarps = kScanners / 32;
+template <int STAGERS, int SCANNER_REGS, int STAGER_REGS>
+struct ScanTeam {
+  static constexpr int kStagers = STAGERS, kBlock = kScanners + STAGERS;
+  static constexpr int kScannerRegs = SCANNER_REGS, kStagerRegs = STAGER_REGS;
+  static constexpr int kLaunchRegs = 65536 / 2 / kBlock / 8 * 8;
+  static_assert(kScanners * SCANNER_REGS + STAGERS * STAGER_REGS <= kBlock * kLaunchRegs, "more registers than launched with");
+};
+// Forward, eight staging warps with little each keep up with the scanners (238 us
+// for 8 x 2048 x 2048 channels with 16 states in bf16; with four 243).  Backward,
+// four are enough and leave the scanners more registers (762 us; with eight, which
+// spill, 827).
+using ForwardTeam = ScanTeam<256, 112, 64>;
+using BackwardTeam = ScanTeam<128, 136, 120>;
 
 template <int N>
 __device__ __forceinline__ void more_registers() {
@@ -59,18 +65,21 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-template <int S>
+template <int S, class TEAM>
 struct ScanShape {
   static constexpr int kStates = 4 * S;                     // padded number of states
   static constexpr int kWarpCh = 2 * (32 / S);              // channels per scanning warp
   static constexpr int kCh = kScanWarps * kWarpCh;          // channels per block
-  static constexpr int kRowThreads = kStagers / kTile;      // threads that stage one step: 16
-  static constexpr int kE = kCh / kRowThreads;              // neighbouring channels a thread stages: 8, 4, 2, 1
+  static constexpr int kRowThreads = TEAM::kStagers / kTile;  // threads that stage one step
+  static constexpr int kE = kCh / kRowThreads;              // neighbouring channels a thread stages
   static constexpr int kN = (kStates + kRowThreads - 1) / kRowThreads;  // states a thread stages
 };
 
 // The whole block meets; scanners and stagers call it from their own code.
-__device__ __forceinline__ void meet() { asm volatile("barrier.sync 1, %0;" ::"n"(kBlock) : "memory"); }
+template <class TEAM>
+__device__ __forceinline__ void meet() {
+  asm volatile("barrier.sync 1, %0;" ::"n"(TEAM::kBlock) : "memory");
+}
 
 // Strides, sizes and flags as the kernels use them.
 struct ScanDims {
@@ -79,9 +88,9 @@ struct ScanDims {
 };
 
 // A scanning thread's place: 2 channels, 4 states.
-template <int S>
+template <int S, class TEAM>
 struct Scanner {
-  using P = ScanShape<S>;
+  using P = ScanShape<S, TEAM>;
   int lane, warp, slice, cl, s0, c, mine;  // cl: channel pair in the block, c: of all channels, mine: of the pair that exist
   __device__ __forceinline__ Scanner(int tid, int c0, int nch) {
     lane = tid & 31, warp = tid >> 5, slice = lane & (S - 1);
@@ -92,9 +101,10 @@ struct Scanner {
 };
 
 // A staging thread's place: one step of the tile, kE channels.
-template <int S>
+template <int S, class TEAM>
 struct Stager {
-  using P = ScanShape<S>;
+  using P = ScanShape<S, TEAM>;
+  static constexpr int kPairs = (P::kE + 1) / 2;
   int tr, pr, col, c, n;  // tr: step, pr: place in the row, col: first channel in the block, c: of all, n: channels that exist
   __device__ __forceinline__ Stager(int tid, int c0, int nch) {
     tr = tid / P::kRowThreads, pr = tid % P::kRowThreads;
@@ -102,16 +112,30 @@ struct Stager {
     c = c0 + col;
     n = max(0, min(P::kE, nch - col));
   }
-  __device__ __forceinline__ void params(const float* p, float (&out)[P::kE]) const {
+  __device__ __forceinline__ void params(const float* p, F2 (&out)[kPairs]) const {
 #pragma unroll
-    for (int i = 0; i < P::kE; ++i) out[i] = p && i < n ? __ldg(p + c + i) : 0.f;
+    for (int i = 0; i < kPairs; ++i)
+      out[i] = pack2(p && 2 * i < n ? __ldg(p + c + 2 * i) : 0.f, p && 2 * i + 1 < n ? __ldg(p + c + 2 * i + 1) : 0.f);
   }
 };
 
+// A tensor's rows as a staging thread meets them, one tile after the other: the
+// address moves on by a constant, instead of being made anew from strides.
+template <class T>
+struct Walk {
+  const T* p;
+  long long by;
+  __device__ __forceinline__ Walk(const void* base, long long first, long long step, int tiles) {
+    p = static_cast<const T*>(base) + first;
+    by = step * (tiles * kTile);
+  }
+  __device__ __forceinline__ void on() { p += by; }
+};
+
 // One step's B or C row on its way to shared memory.
-template <class T, int S>
+template <class T, int S, class TEAM>
 struct StateRow {
-  using P = ScanShape<S>;
+  using P = ScanShape<S, TEAM>;
   T v[P::kN];
   __device__ __forceinline__ void load(const T* row, int n, bool live, int k) {
 #pragma unroll
@@ -139,8 +163,8 @@ __device__ __forceinline__ int scan_row_length(const pt_scan_args& a, int b) {
 using Quad = F2[2][2];
 
 // A state array [dim, state] in global memory (fp32): this thread's values.
-template <int S>
-__device__ __forceinline__ void load_states(const float* p, const pt_scan_args& a, const Scanner<S>& me, Quad& h) {
+template <int S, class TEAM>
+__device__ __forceinline__ void load_states(const float* p, const pt_scan_args& a, const Scanner<S, TEAM>& me, Quad& h) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float* q = p + static_cast<long long>(me.c + i) * a.state + me.s0;
@@ -155,8 +179,8 @@ __device__ __forceinline__ void load_states(const float* p, const pt_scan_args& 
     }
   }
 }
-template <int S>
-__device__ __forceinline__ void store_states(float* p, const pt_scan_args& a, const Scanner<S>& me, const Quad& h) {
+template <int S, class TEAM>
+__device__ __forceinline__ void store_states(float* p, const pt_scan_args& a, const Scanner<S, TEAM>& me, const Quad& h) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float* q = p + static_cast<long long>(me.c + i) * a.state + me.s0;
@@ -172,8 +196,8 @@ __device__ __forceinline__ void store_states(float* p, const pt_scan_args& a, co
 }
 
 // Decay rates times log2 e: exp(delta A) = 2^(delta A2).
-template <int S>
-__device__ __forceinline__ void load_rates(const pt_scan_args& a, const Scanner<S>& me, Quad& A2) {
+template <int S, class TEAM>
+__device__ __forceinline__ void load_rates(const pt_scan_args& a, const Scanner<S, TEAM>& me, Quad& A2) {
   load_states(a.A, a, me, A2);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -221,7 +245,7 @@ __device__ __forceinline__ void sum_slices(float (&v)[2][2], int slice, float& f
 }
 // Writes what sum_slices left, to rows i and i + 1 of dst.
 template <int S>
-__device__ __forceinline__ void put_sums(float (*dst)[ScanShape<S>::kCh], int i, int cl, int slice, float first,
+__device__ __forceinline__ void put_sums(float (*dst)[64 / S * kScanWarps], int i, int cl, int slice, float first,
                                          float second) {
   if constexpr (S == 2) {
     dst[i][cl + slice] = first;
@@ -240,17 +264,17 @@ __device__ __forceinline__ float dot2(F2 h, F2 c, float s, int first, int states
 }
 
 // Where a block works.
-template <int S>
+template <int S, class TEAM>
 struct ScanBlock {
   int cb, rest, g, c0, nch;  // block of channels, index of the rest of the grid, group, first channel, channels
   __device__ __forceinline__ ScanBlock(const pt_scan_args& a, int cblocks) {
     const int nblk = cblocks * a.groups;
     cb = static_cast<int>(blockIdx.x) % nblk;
     rest = static_cast<int>(blockIdx.x) / nblk;
-    const int per = a.dim / a.groups, first = (cb % cblocks) * ScanShape<S>::kCh;
+    const int per = a.dim / a.groups, first = (cb % cblocks) * 64 / S * kScanWarps;
     g = cb / cblocks;
     c0 = g * per + first;
-    nch = min(ScanShape<S>::kCh, per - first);
+    nch = min(64 / S * kScanWarps, per - first);
   }
 };
 
@@ -258,20 +282,21 @@ struct ScanBlock {
 // Forward (REV false): the state that a segment reaches from zero, and the sum
 // of its deltas.  Backward: the gradient a_t dh_t that leaves the segment at
 // its start when none enters at its end.
-template <int S>
+template <int S, class TEAM>
 struct SegmentSmem {
-  using P = ScanShape<S>;
+  using P = ScanShape<S, TEAM>;
   float d[2][kTile][P::kCh], v[2][kTile][P::kCh];  // delta; delta x or dout silu(z)
   float B[2][kTile][P::kStates];
 };
 
 template <class T, int S, bool REV>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(ForwardTeam::kBlock, 2)
     seq_scan_segment_kernel(pt_scan_args a, ScanDims dm, float* seg_h, float* seg_d) {
-  using P = ScanShape<S>;
+  using TEAM = ForwardTeam;
+  using P = ScanShape<S, TEAM>;
   extern __shared__ __align__(16) unsigned char smem[];
-  auto& sm = *reinterpret_cast<SegmentSmem<S>*>(smem);
-  const ScanBlock<S> at(a, dm.cblocks);
+  auto& sm = *reinterpret_cast<SegmentSmem<S, TEAM>*>(smem);
+  const ScanBlock<S, TEAM> at(a, dm.cblocks);
   // The last segment (backward: the first) has none to hand its state to.
   const int seg = at.rest % (dm.segs - 1) + (REV ? 1 : 0), b = at.rest / (dm.segs - 1);
   const int len = scan_row_length(a, b);
@@ -280,62 +305,76 @@ __global__ void __launch_bounds__(kBlock, 2)
   auto tile_of = [&](int k) { return t0 + (REV ? tiles - 1 - k : k) * kTile; };
   const int tid = static_cast<int>(threadIdx.x);
   if (tid >= kScanners) {
-    fewer_registers<kFwdStagerRegs>();
-    const Stager<S> me(tid - kScanners, at.c0, at.nch);
-    float bias[P::kE];
+    fewer_registers<TEAM::kStagerRegs>();
+    const Stager<S, TEAM> me(tid - kScanners, at.c0, at.nch);
+    F2 bias[me.kPairs];
     me.params(a.dt_bias, bias);
     Pack<T, P::kE> dt, in, z;
-    StateRow<T, S> row;
-    auto load = [&](int k) {
-      const int t = tile_of(k) + me.tr;
-      const bool live = t < len && t < t1;
+    StateRow<T, S, TEAM> row;
+    const int end = min(len, t1), way = REV ? -1 : 1;
+    int t = tile_of(0) + me.tr, t_in = t;  // of the tile to load, of the one loaded last
+    const void* in_base = REV ? a.dy : a.x;
+    const long long in_batch = REV ? a.dy_batch : a.x_batch, in_step = REV ? a.dy_step : a.x_step;
+    Walk<T> wdt(a.dt, b * a.dt_batch + t * a.dt_step + me.c, a.dt_step, way);
+    Walk<T> win(in_base, b * in_batch + t * in_step + me.c, in_step, way);
+    Walk<T> wz(a.z, a.z ? b * a.z_batch + t * a.z_step + me.c : 0, a.z_step, way);
+    Walk<T> wrow(REV ? a.C : a.B,
+                 REV ? b * a.C_batch + t * a.C_step + at.g * a.C_group : b * a.B_batch + t * a.B_step + at.g * a.B_group,
+                 REV ? a.C_step : a.B_step, way);
+    const bool gated = REV && a.z;
+    auto load = [&]() {
+      const bool live = t < end;
       if (live) {
-        dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
-        if constexpr (REV) {
-          in.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + me.c, me.n, dm.wide & 8);
-          if (a.z) z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
-        } else {
-          in.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
-        }
+        dt.load(wdt.p, me.n, dm.wide & 2);
+        in.load(win.p, me.n, dm.wide & (REV ? 8 : 1));
+        if (gated) z.load(wz.p, me.n, dm.wide & 4);
       }
-      row.load(REV ? static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group
-                   : static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group,
-               a.state, live, me.pr);
+      row.load(wrow.p, a.state, live, me.pr);
+      t_in = t;
+      t += way * kTile;
+      wdt.on(), win.on(), wz.on(), wrow.on();
     };
     auto convert = [&](int k) {
-      const int t = tile_of(k) + me.tr;
-      float d[P::kE] = {}, v[P::kE] = {};
-      if (t < len && t < t1) {
+      F2 d[me.kPairs] = {}, v[me.kPairs] = {};
+      if (t_in < end) {
 #pragma unroll
-        for (int i = 0; i < P::kE; ++i) {
-          const float raw = dt.f(i) + bias[i];
-          d[i] = a.dt_softplus ? softplusf(raw) : raw;
-          v[i] = REV ? (a.z ? in.f(i) * siluf(z.f(i)) : in.f(i)) : d[i] * in.f(i);
+        for (int i = 0; i < me.kPairs; ++i) {
+          d[i] = add2(dt.pair(i), bias[i]);
+          if (a.dt_softplus) d[i] = softplus2(d[i]);
+          v[i] = in.pair(i);
+          if constexpr (REV) {
+            if (gated) {
+              const F2 zi = z.pair(i);
+              v[i] = mul2(v[i], mul2(zi, sigmoid2(zi)));
+            }
+          } else {
+            v[i] = mul2(v[i], d[i]);
+          }
         }
       }
-      put_floats<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
-      put_floats<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
+      put_pairs<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
+      put_pairs<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
       row.store(sm.B[k & 1][me.tr], me.pr);
     };
     if (tiles > 0) {
-      load(0);
+      load();
       convert(0);
-      if (tiles > 1) load(1);
+      if (tiles > 1) load();
     }
-    meet();
+    meet<TEAM>();
     for (int k = 0; k < tiles; ++k) {
       if (k + 1 < tiles) convert(k + 1);
-      if (k + 2 < tiles) load(k + 2);
-      meet();
+      if (k + 2 < tiles) load();
+      meet<TEAM>();
     }
     return;
   }
-  more_registers<kFwdScannerRegs>();
-  const Scanner<S> me(tid, at.c0, at.nch);
+  more_registers<TEAM::kScannerRegs>();
+  const Scanner<S, TEAM> me(tid, at.c0, at.nch);
   Quad A2, h = {};
   float dsum[2] = {0.f, 0.f};
   load_rates(a, me, A2);
-  meet();
+  meet<TEAM>();
   for (int k = 0; k < tiles; ++k) {
     const int st = k & 1;
 #pragma unroll 8
@@ -353,7 +392,7 @@ __global__ void __launch_bounds__(kBlock, 2)
         }
       }
     }
-    meet();
+    meet<TEAM>();
   }
   const long long out = static_cast<long long>(b) * dm.segs + seg;
   store_states(seg_h + out * a.dim * a.state, a, me, h);
@@ -364,9 +403,9 @@ __global__ void __launch_bounds__(kBlock, 2)
 }
 
 // h <- exp(A sum delta of segment s) h + its own state.
-template <int S>
+template <int S, class TEAM>
 __device__ __forceinline__ void join_segment(const pt_scan_args& a, const ScanDims& dm, const float* seg_h,
-                                             const float* seg_d, int b, int s, const Scanner<S>& me, const Quad& A2,
+                                             const float* seg_d, int b, int s, const Scanner<S, TEAM>& me, const Quad& A2,
                                              Quad& h) {
   const long long row = static_cast<long long>(b) * dm.segs + s;
   Quad l;
@@ -380,106 +419,122 @@ __device__ __forceinline__ void join_segment(const pt_scan_args& a, const ScanDi
 }
 
 // ---------------------------------------------------------------- forward
-template <int S>
+template <int S, class TEAM>
 struct ForwardSmem {
-  using P = ScanShape<S>;
+  using P = ScanShape<S, TEAM>;
   float d[2][kTile][P::kCh], v[2][kTile][P::kCh], y[2][kTile][P::kCh];  // delta, delta x, sums over states of h C
   float B[2][kTile][P::kStates], C[2][kTile][P::kStates];
 };
 
 template <class T, int S, bool PAD>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(ForwardTeam::kBlock, 2)
     seq_scan_fwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d) {
-  using P = ScanShape<S>;
+  using TEAM = ForwardTeam;
+  using P = ScanShape<S, TEAM>;
   extern __shared__ __align__(16) unsigned char smem[];
-  auto& sm = *reinterpret_cast<ForwardSmem<S>*>(smem);
-  const ScanBlock<S> at(a, dm.cblocks);
+  auto& sm = *reinterpret_cast<ForwardSmem<S, TEAM>*>(smem);
+  const ScanBlock<S, TEAM> at(a, dm.cblocks);
   const int seg = at.rest % dm.segs, b = at.rest / dm.segs;
   const int len = scan_row_length(a, b);
   const int t0 = seg * dm.seg_len, t1 = min(t0 + dm.seg_len, a.len);
   const int tiles = max(0, (t1 - t0 + kTile - 1) / kTile);
   const int tid = static_cast<int>(threadIdx.x);
   if (tid >= kScanners) {
-    fewer_registers<kFwdStagerRegs>();
-    const Stager<S> me(tid - kScanners, at.c0, at.nch);
-    float bias[P::kE], Dv[P::kE];
+    fewer_registers<TEAM::kStagerRegs>();
+    const Stager<S, TEAM> me(tid - kScanners, at.c0, at.nch);
+    F2 bias[me.kPairs], Dv[me.kPairs];
     me.params(a.dt_bias, bias);
     me.params(a.D, Dv);
     // x and z of three tiles: the one whose outputs are next, the one being scanned, the next one.
     Pack<T, P::kE> dt, x[3], z[3];
-    StateRow<T, S> rowB, rowC;
-    auto load = [&](int k) {
-      const int t = t0 + k * kTile + me.tr;
-      const bool live = t < len && t < t1;
+    StateRow<T, S, TEAM> rowB, rowC;
+    const int end = min(len, t1);
+    int t = t0 + me.tr;  // of the tile to load; t_in of the one to convert, t_out of the one to write
+    int t_in = t, t_out = t;
+    Walk<T> wdt(a.dt, b * a.dt_batch + t * a.dt_step + me.c, a.dt_step, 1);
+    Walk<T> wx(a.x, b * a.x_batch + t * a.x_step + me.c, a.x_step, 1);
+    Walk<T> wz(a.z, a.z ? b * a.z_batch + t * a.z_step + me.c : 0, a.z_step, 1);
+    Walk<T> wB(a.B, b * a.B_batch + t * a.B_step + at.g * a.B_group, a.B_step, 1);
+    Walk<T> wC(a.C, b * a.C_batch + t * a.C_step + at.g * a.C_group, a.C_step, 1);
+    T* y_out = static_cast<T*>(a.y) + (static_cast<long long>(b) * a.len + t) * a.dim + me.c;
+    auto load = [&]() {
+      const bool live = t < end;
       if (live) {
-        dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
-        x[2].load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
-        if (a.z) z[2].load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
+        dt.load(wdt.p, me.n, dm.wide & 2);
+        x[2].load(wx.p, me.n, dm.wide & 1);
+        if (a.z) z[2].load(wz.p, me.n, dm.wide & 4);
       }
-      rowB.load(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live, me.pr);
-      rowC.load(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live, me.pr);
+      rowB.load(wB.p, a.state, live, me.pr);
+      rowC.load(wC.p, a.state, live, me.pr);
+      t += kTile;
+      wdt.on(), wx.on(), wz.on(), wB.on(), wC.on();
     };
     auto convert = [&](int k) {
-      const int t = t0 + k * kTile + me.tr;
       x[0] = x[1], z[0] = z[1], x[1] = x[2], z[1] = z[2];
-      float d[P::kE] = {}, v[P::kE] = {};
-      if (t < len && t < t1) {
+      F2 d[me.kPairs] = {}, v[me.kPairs] = {};
+      if (t_in < end) {
 #pragma unroll
-        for (int i = 0; i < P::kE; ++i) {
-          const float raw = dt.f(i) + bias[i];
-          d[i] = a.dt_softplus ? softplusf(raw) : raw;
-          v[i] = d[i] * x[1].f(i);
+        for (int i = 0; i < me.kPairs; ++i) {
+          d[i] = add2(dt.pair(i), bias[i]);
+          if (a.dt_softplus) d[i] = softplus2(d[i]);
+          v[i] = mul2(d[i], x[1].pair(i));
         }
       }
-      put_floats<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
-      put_floats<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
+      put_pairs<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
+      put_pairs<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
       rowB.store(sm.B[k & 1][me.tr], me.pr);
       rowC.store(sm.C[k & 1][me.tr], me.pr);
+      t_in += kTile;
     };
-    auto finish = [&](int k, const Pack<T, P::kE>& xk, const Pack<T, P::kE>& zk) {
-      const int t = t0 + k * kTile + me.tr;
-      if (t >= t1) return;
-      Pack<T, P::kE> out;
-      out.zero();
-      if (t < len) {
-        float y[P::kE];
-        get_floats<P::kE>(&sm.y[k & 1][me.tr][me.col], y);
+    auto finish = [&](int k) {
+      if (t_out < t1) {
+        Pack<T, P::kE> out;
+        out.zero();
+        if (t_out < len) {
+          F2 y[me.kPairs];
+          get_pairs<P::kE>(&sm.y[k & 1][me.tr][me.col], y);
 #pragma unroll
-        for (int i = 0; i < P::kE; ++i) {
-          if (a.D) y[i] = fmaf(Dv[i], xk.f(i), y[i]);
-          if (a.z) y[i] *= siluf(zk.f(i));
-          out.set(i, y[i]);
+          for (int i = 0; i < me.kPairs; ++i) {
+            if (a.D) y[i] = fma2(Dv[i], x[0].pair(i), y[i]);
+            if (a.z) {
+              const F2 zi = z[0].pair(i);
+              y[i] = mul2(y[i], mul2(zi, sigmoid2(zi)));
+            }
+            out.set_pair(i, y[i]);
+          }
         }
+        out.store(y_out, me.n, dm.wide & 16);
       }
-      out.store(static_cast<T*>(a.y) + (static_cast<long long>(b) * a.len + t) * a.dim + me.c, me.n, dm.wide & 16);
+      t_out += kTile;
+      y_out += static_cast<long long>(kTile) * a.dim;
     };
     if (tiles > 0) {
-      load(0);
+      load();
       convert(0);
-      if (tiles > 1) load(1);
+      if (tiles > 1) load();
     }
-    meet();
+    meet<TEAM>();
     for (int k = 0; k < tiles; ++k) {
-      if (k > 0) finish(k - 1, x[0], z[0]);
+      if (k > 0) finish(k - 1);
       if (k + 1 < tiles) {
         convert(k + 1);
-        if (k + 2 < tiles) load(k + 2);
+        if (k + 2 < tiles) load();
       } else {
         x[0] = x[1], z[0] = z[1];
       }
-      meet();
+      meet<TEAM>();
     }
-    if (tiles > 0) finish(tiles - 1, x[0], z[0]);
+    if (tiles > 0) finish(tiles - 1);
     return;
   }
-  more_registers<kFwdScannerRegs>();
-  const Scanner<S> me(tid, at.c0, at.nch);
+  more_registers<TEAM::kScannerRegs>();
+  const Scanner<S, TEAM> me(tid, at.c0, at.nch);
   Quad A2, h = {};
   load_rates(a, me, A2);
   if (a.h0) load_states(a.h0 + static_cast<long long>(b) * a.dim * a.state, a, me, h);
   for (int s = 0; s < seg; ++s) join_segment(a, dm, seg_h, seg_d, b, s, me, A2, h);
   const long long ckpt_row = (static_cast<long long>(a.len) + kTile - 1) / kTile;
-  meet();
+  meet<TEAM>();
   for (int k = 0; k < tiles; ++k) {
     const int st = k & 1;
     if (a.checkpoints)
@@ -551,7 +606,7 @@ __global__ void __launch_bounds__(kBlock, 2)
       sum_slices<S>(last, me.slice, first, second);
       put_sums<S>(sm.y[st], kTile - 2, me.cl, me.slice, first, second);
     }
-    meet();
+    meet<TEAM>();
   }
   if (a.hlast && seg == dm.segs - 1)
     store_states(a.hlast + static_cast<long long>(b) * a.dim * a.state, a, me, h);
@@ -593,9 +648,9 @@ __device__ __forceinline__ void sum_channels(float (&v)[8], int lane, float* dst
   }
 }
 
-template <int S>
+template <int S, class TEAM>
 struct BackwardSmem {
-  using P = ScanShape<S>;
+  using P = ScanShape<S, TEAM>;
   float d[2][kTile][P::kCh];                          // delta
   float v[2][kTile][P::kCh], w[2][kTile][P::kCh];     // delta x, dout silu(z); then the sums over states of dh B, h C
   float gA[2][kTile][P::kCh];                         // sums over states of (d log a) A2
@@ -608,13 +663,14 @@ struct BackwardSmem {
 };
 
 template <class T, int S, bool PAD>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
     seq_scan_bwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d, float* part_bc,
                         float* part_p) {
-  using P = ScanShape<S>;
+  using TEAM = BackwardTeam;
+  using P = ScanShape<S, TEAM>;
   extern __shared__ __align__(16) unsigned char smem[];
-  auto& sm = *reinterpret_cast<BackwardSmem<S>*>(smem);
-  const ScanBlock<S> at(a, dm.cblocks);
+  auto& sm = *reinterpret_cast<BackwardSmem<S, TEAM>*>(smem);
+  const ScanBlock<S, TEAM> at(a, dm.cblocks);
   const int seg = at.rest % dm.segs, chunk = at.rest / dm.segs;
   const int t0 = seg * dm.seg_len, t1 = min(t0 + dm.seg_len, a.len);
   const int tiles = max(0, (t1 - t0 + kTile - 1) / kTile);
@@ -627,77 +683,90 @@ __global__ void __launch_bounds__(kBlock, 2)
   auto tile_of = [&](int k) { return t0 + (tiles - 1 - k) * kTile; };
 
   if (tid >= kScanners) {
-    fewer_registers<kBwdStagerRegs>();
-    const Stager<S> me(tid - kScanners, at.c0, at.nch);
-    float accD[P::kE] = {}, accb[P::kE] = {};
+    fewer_registers<TEAM::kStagerRegs>();
+    const Stager<S, TEAM> me(tid - kScanners, at.c0, at.nch);
+    F2 bias[me.kPairs], Dv[me.kPairs], accD[me.kPairs] = {}, accb[me.kPairs] = {};
+    me.params(a.dt_bias, bias);
+    me.params(a.D, Dv);
     for (int b = chunk; b < a.batch; b += dm.row_chunks) {
-      const int len = scan_row_length(a, b);
+      const int len = scan_row_length(a, b), end = min(len, t1);
       // A tile takes the scanners far longer than a trip to memory, so nothing is fetched ahead and few registers do.
       Pack<T, P::kE> dt, x, z, dy;
-      auto load = [&](int k) {
-        const int t = tile_of(k) + me.tr;
-        if (t < len && t < t1) {
-          dt.load(static_cast<const T*>(a.dt) + b * a.dt_batch + t * a.dt_step + me.c, me.n, dm.wide & 2);
-          x.load(static_cast<const T*>(a.x) + b * a.x_batch + t * a.x_step + me.c, me.n, dm.wide & 1);
-          dy.load(static_cast<const T*>(a.dy) + b * a.dy_batch + t * a.dy_step + me.c, me.n, dm.wide & 8);
-          if (a.z) z.load(static_cast<const T*>(a.z) + b * a.z_batch + t * a.z_step + me.c, me.n, dm.wide & 4);
-        }
+      int t_in = tile_of(0) + me.tr, t_out = t_in;  // of the tile to convert, of the one whose gradients are next
+      Walk<T> wdt(a.dt, b * a.dt_batch + t_in * a.dt_step + me.c, a.dt_step, -1);
+      Walk<T> wx(a.x, b * a.x_batch + t_in * a.x_step + me.c, a.x_step, -1);
+      Walk<T> wdy(a.dy, b * a.dy_batch + t_in * a.dy_step + me.c, a.dy_step, -1);
+      Walk<T> wz(a.z, a.z ? b * a.z_batch + t_in * a.z_step + me.c : 0, a.z_step, -1);
+      Walk<T> wB(a.B, b * a.B_batch + t_in * a.B_step + at.g * a.B_group, a.B_step, -1);
+      Walk<T> wC(a.C, b * a.C_batch + t_in * a.C_step + at.g * a.C_group, a.C_step, -1);
+      long long o = (static_cast<long long>(b) * a.len + t_out) * a.dim + me.c;  // gradients of t_out
+      // The inputs of a tile, `back` tiles behind the walk.
+      auto load = [&](int back) {
+        dt.load(wdt.p - back * wdt.by, me.n, dm.wide & 2);
+        x.load(wx.p - back * wx.by, me.n, dm.wide & 1);
+        dy.load(wdy.p - back * wdy.by, me.n, dm.wide & 8);
+        if (a.z) z.load(wz.p - back * wz.by, me.n, dm.wide & 4);
       };
       auto convert = [&](int k) {
-        const int t = tile_of(k) + me.tr;
-        const bool live = t < len && t < t1;
-        load(k);
-        StateRow<T, S> rowB, rowC;
-        rowB.load(static_cast<const T*>(a.B) + b * a.B_batch + t * a.B_step + at.g * a.B_group, a.state, live, me.pr);
-        rowC.load(static_cast<const T*>(a.C) + b * a.C_batch + t * a.C_step + at.g * a.C_group, a.state, live, me.pr);
-        float d[P::kE] = {}, v[P::kE] = {}, w[P::kE] = {};
+        const bool live = t_in < end;
+        StateRow<T, S, TEAM> rowB, rowC;
+        rowB.load(wB.p, a.state, live, me.pr);
+        rowC.load(wC.p, a.state, live, me.pr);
+        F2 d[me.kPairs] = {}, v[me.kPairs] = {}, w[me.kPairs] = {};
         if (live) {
+          load(0);
 #pragma unroll
-          for (int i = 0; i < P::kE; ++i) {
-            const float raw = dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f);
-            d[i] = a.dt_softplus ? softplusf(raw) : raw;
-            v[i] = d[i] * x.f(i);
-            w[i] = a.z ? dy.f(i) * siluf(z.f(i)) : dy.f(i);
-          }
-        }
-        put_floats<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
-        put_floats<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
-        put_floats<P::kE>(&sm.w[k & 1][me.tr][me.col], w);
-        rowB.store(sm.B[k & 1][me.tr], me.pr);
-        rowC.store(sm.C[k & 1][me.tr], me.pr);
-      };
-      auto finish = [&](int k) {
-        const int tile = tile_of(k), t = tile + me.tr, st = k & 1;
-        if (t < t1) {
-          load(k);
-          Pack<T, P::kE> ox, odt, oz;
-          ox.zero(), odt.zero(), oz.zero();
-          if (t < len) {
-            float d[P::kE], gB[P::kE], gA[P::kE], y[P::kE];
-            get_floats<P::kE>(&sm.d[st][me.tr][me.col], d);
-            get_floats<P::kE>(&sm.v[st][me.tr][me.col], gB);
-            get_floats<P::kE>(&sm.gA[st][me.tr][me.col], gA);
-            get_floats<P::kE>(&sm.w[st][me.tr][me.col], y);
-#pragma unroll
-            for (int i = 0; i < P::kE; ++i) {
-              const float xv = x.f(i), dyv = dy.f(i);
-              const float Dv = a.D && i < me.n ? __ldg(a.D + me.c + i) : 0.f;
-              float w = dyv;
-              if (a.z) {
-                const float zv = z.f(i), s = sigmoidf(zv);
-                w *= zv * s;
-                oz.set(i, dyv * (a.D ? fmaf(Dv, xv, y[i]) : y[i]) * silu_grad(zv, s));
-              }
-              float gd = fmaf(gB[i], xv, gA[i] * kLn2);
-              if (a.dt_softplus)
-                gd *= sigmoidf(dt.f(i) + (a.dt_bias && i < me.n ? __ldg(a.dt_bias + me.c + i) : 0.f));
-              ox.set(i, a.D ? fmaf(Dv, w, gB[i] * d[i]) : gB[i] * d[i]);
-              odt.set(i, gd);
-              accD[i] = fmaf(w, xv, accD[i]);
-              accb[i] += gd;
+          for (int i = 0; i < me.kPairs; ++i) {
+            d[i] = add2(dt.pair(i), bias[i]);
+            if (a.dt_softplus) d[i] = softplus2(d[i]);
+            v[i] = mul2(d[i], x.pair(i));
+            w[i] = dy.pair(i);
+            if (a.z) {
+              const F2 zi = z.pair(i);
+              w[i] = mul2(w[i], mul2(zi, sigmoid2(zi)));
             }
           }
-          const long long o = (static_cast<long long>(b) * a.len + t) * a.dim + me.c;
+        }
+        put_pairs<P::kE>(&sm.d[k & 1][me.tr][me.col], d);
+        put_pairs<P::kE>(&sm.v[k & 1][me.tr][me.col], v);
+        put_pairs<P::kE>(&sm.w[k & 1][me.tr][me.col], w);
+        rowB.store(sm.B[k & 1][me.tr], me.pr);
+        rowC.store(sm.C[k & 1][me.tr], me.pr);
+        t_in -= kTile;
+        wdt.on(), wx.on(), wdy.on(), wz.on(), wB.on(), wC.on();
+      };
+      auto finish = [&](int k, int back) {
+        const int st = k & 1;
+        if (t_out < t1) {
+          Pack<T, P::kE> ox, odt, oz;
+          ox.zero(), odt.zero(), oz.zero();
+          if (t_out < len) {
+            load(back);
+            F2 d[me.kPairs], gB[me.kPairs], gA[me.kPairs], y[me.kPairs];
+            get_pairs<P::kE>(&sm.d[st][me.tr][me.col], d);
+            get_pairs<P::kE>(&sm.v[st][me.tr][me.col], gB);
+            get_pairs<P::kE>(&sm.gA[st][me.tr][me.col], gA);
+            get_pairs<P::kE>(&sm.w[st][me.tr][me.col], y);
+#pragma unroll
+            for (int i = 0; i < me.kPairs; ++i) {
+              const F2 xv = x.pair(i), dyv = dy.pair(i);
+              F2 w = dyv;
+              if (a.z) {
+                const F2 zv = z.pair(i), s = sigmoid2(zv);
+                w = mul2(w, mul2(zv, s));
+                const F2 yv = a.D ? fma2(Dv[i], xv, y[i]) : y[i];
+                oz.set_pair(i, mul2(mul2(dyv, yv), silu_grad2(zv, s)));
+              }
+              F2 gd = fma2(gB[i], xv, mul2(gA[i], same2(kLn2)));
+              if (a.dt_softplus) gd = mul2(gd, sigmoid2(add2(dt.pair(i), bias[i])));
+              F2 gx = mul2(gB[i], d[i]);
+              if (a.D) gx = fma2(Dv[i], w, gx);
+              ox.set_pair(i, gx);
+              odt.set_pair(i, gd);
+              accD[i] = fma2(w, xv, accD[i]);
+              accb[i] = add2(accb[i], gd);
+            }
+          }
           const bool wide = dm.wide & 16;
           if (a.dx) ox.store(static_cast<T*>(a.dx) + o, me.n, wide);
           if (a.ddt) odt.store(static_cast<T*>(a.ddt) + o, me.n, wide);
@@ -705,33 +774,38 @@ __global__ void __launch_bounds__(kBlock, 2)
         }
         if (part_bc) {
           // [block of the group's channels][batch][len][group][2 * states]
-          const int n = min(kTile, t1 - tile) * 2 * P::kStates;
+          constexpr int kRow = 2 * P::kStates, kEach = 4;
+          const int tile = t_out - me.tr, rows = min(kTile, t1 - tile);
           const long long row = (static_cast<long long>(at.cb % dm.cblocks) * a.batch + b) * a.len + tile;
-#pragma unroll 4
-          for (int i = tid - kScanners; i < kTile * 2 * P::kStates; i += kStagers) {
-            if (i >= n) break;
-            const int q = i / (2 * P::kStates), k2 = i % (2 * P::kStates);
-            float s = 0.f;
+#pragma unroll 1
+          for (int i = (tid - kScanners) * kEach; i < rows * kRow; i += TEAM::kStagers * kEach) {
+            const int q = i / kRow, k2 = i % kRow;
+            float4 s = *reinterpret_cast<const float4*>(&sm.red[st][0][q][k2]);
 #pragma unroll
-            for (int w = 0; w < kScanWarps; ++w) s += sm.red[st][w][q][k2];
-            part_bc[((row + q) * a.groups + at.g) * (2 * P::kStates) + k2] = s;
+            for (int w = 1; w < kScanWarps; ++w) {
+              const float4 m = *reinterpret_cast<const float4*>(&sm.red[st][w][q][k2]);
+              s.x += m.x, s.y += m.y, s.z += m.z, s.w += m.w;
+            }
+            *reinterpret_cast<float4*>(part_bc + ((row + q) * a.groups + at.g) * kRow + k2) = s;
           }
         }
+        t_out -= kTile;
+        o -= static_cast<long long>(kTile) * a.dim;
       };
       if (tiles > 0) convert(0);
-      meet();
+      meet<TEAM>();
       for (int k = 0; k < tiles; ++k) {
-        if (k > 0) finish(k - 1);
+        if (k > 0) finish(k - 1, 2);  // the walk is at tile k + 1
         if (k + 1 < tiles) convert(k + 1);
-        meet();
+        meet<TEAM>();
       }
-      if (tiles > 0) finish(tiles - 1);
-      meet();
+      if (tiles > 0) finish(tiles - 1, 1);
+      meet<TEAM>();
     }
-    put_floats<P::kE>(&sm.accD[me.tr][me.col], accD);
-    put_floats<P::kE>(&sm.accb[me.tr][me.col], accb);
-    meet();
-    for (int c = tid - kScanners; c < at.nch; c += kStagers) {
+    put_pairs<P::kE>(&sm.accD[me.tr][me.col], accD);
+    put_pairs<P::kE>(&sm.accb[me.tr][me.col], accb);
+    meet<TEAM>();
+    for (int c = tid - kScanners; c < at.nch; c += TEAM::kStagers) {
       float sD = 0.f, sb = 0.f;
 #pragma unroll
       for (int q = 0; q < kTile; ++q) sD += sm.accD[q][c], sb += sm.accb[q][c];
@@ -741,8 +815,8 @@ __global__ void __launch_bounds__(kBlock, 2)
     return;
   }
 
-  more_registers<kBwdScannerRegs>();
-  const Scanner<S> me(tid, at.c0, at.nch);
+  more_registers<TEAM::kScannerRegs>();
+  const Scanner<S, TEAM> me(tid, at.c0, at.nch);
   Quad A2;
   load_rates(a, me, A2);
   sm.accA[0][tid] = sm.accA[1][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -771,7 +845,7 @@ __global__ void __launch_bounds__(kBlock, 2)
     Quad g = {};  // a_{t+1} dh_{t+1}
     if (a.dhlast) load_states(a.dhlast + b * all, a, me, g);
     for (int s = dm.segs - 1; s > seg; --s) join_segment(a, dm, seg_h, seg_d, b, s, me, A2, g);
-    meet();
+    meet<TEAM>();
     for (int k = 0; k < tiles; ++k) {
       const int st = k & 1;
       Quad first, h;  // the state at the tile's start, and walking on from it
@@ -879,10 +953,10 @@ __global__ void __launch_bounds__(kBlock, 2)
         s.x += lo2(dA[c][0]), s.y += hi2(dA[c][0]), s.z += lo2(dA[c][1]), s.w += hi2(dA[c][1]);
         sm.accA[c][tid] = s;
       }
-      meet();
+      meet<TEAM>();
     }
     if (a.dh0 && seg == 0) store_states(a.dh0 + b * all, a, me, g);
-    meet();  // the next row's tiles overwrite what this row's last gradients are made from
+    meet<TEAM>();  // the next row's tiles overwrite what this row's last gradients are made from
   }
   if (a.dA) {
     Quad dA;
@@ -893,7 +967,7 @@ __global__ void __launch_bounds__(kBlock, 2)
     }
     store_states(mine, a, me, dA);
   }
-  meet();
+  meet<TEAM>();
 }
 
 // dB and dC from the blocks' partial sums, in block order.
@@ -979,9 +1053,9 @@ cudaError_t by_slices(int s, F&& fn) {
   }
 }
 
-template <class T, int S>
+template <class T, int S, class TEAM>
 ScanDims scan_dims(const pt_scan_args& a, const ScanPlan& p) {
-  using P = ScanShape<S>;
+  using P = ScanShape<S, TEAM>;
   constexpr int word = Pack<T, P::kE>::kWord, per = word / static_cast<int>(sizeof(T));
   const bool rows = (a.dim / a.groups) % per == 0;
   auto ok = [&](const void* q, long long s0, long long s1) {
@@ -1004,19 +1078,19 @@ inline size_t segment_floats(const pt_scan_args& a, const ScanPlan& p) {
 }
 
 // Launches a kernel whose shared memory is one Smem.
-template <class Smem, class K, class... A>
-cudaError_t launch_with(K kernel, long long grid, int threads, cudaStream_t stream, A... args) {
+template <class TEAM, class Smem, class K, class... A>
+cudaError_t launch_with(K kernel, long long grid, cudaStream_t stream, A... args) {
   constexpr int bytes = static_cast<int>(sizeof(Smem));
   // The scanners wait for the registers that the split promises them: without those, no launch.
   cudaFuncAttributes attr;
   const cudaError_t known = cudaFuncGetAttributes(&attr, kernel);
   if (known != cudaSuccess) return known;
-  if (attr.numRegs < kLaunchRegs) return cudaErrorLaunchOutOfResources;
+  if (attr.numRegs < TEAM::kLaunchRegs) return cudaErrorLaunchOutOfResources;
   if (bytes > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
   }
-  kernel<<<static_cast<unsigned>(grid), threads, bytes, stream>>>(args...);
+  kernel<<<static_cast<unsigned>(grid), TEAM::kBlock, bytes, stream>>>(args...);
   return cudaGetLastError();
 }
 
@@ -1024,18 +1098,18 @@ template <class T>
 cudaError_t scan_fwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaStream_t stream) {
   return by_slices(p.slices, [&](auto sc) -> cudaError_t {
     constexpr int S = decltype(sc)::value;
-    const ScanDims dm = scan_dims<T, S>(a, p);
+    const ScanDims dm = scan_dims<T, S, ForwardTeam>(a, p);
     float* seg_h = ws;
     float* seg_d = ws + static_cast<size_t>(a.batch) * p.segs * a.dim * a.state;
     const long long blocks = static_cast<long long>(p.cblocks) * a.groups * a.batch;
     if (blocks * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     if (p.segs > 1) {
-      const cudaError_t e = launch_with<SegmentSmem<S>>(
-          seq_scan_segment_kernel<T, S, false>, blocks * (p.segs - 1), kBlock, stream, a, dm, seg_h, seg_d);
+      const cudaError_t e = launch_with<ForwardTeam, SegmentSmem<S, ForwardTeam>>(
+          seq_scan_segment_kernel<T, S, false>, blocks * (p.segs - 1), stream, a, dm, seg_h, seg_d);
       if (e != cudaSuccess) return e;
     }
     auto kernel = a.state == 4 * S ? seq_scan_fwd_kernel<T, S, false> : seq_scan_fwd_kernel<T, S, true>;
-    return launch_with<ForwardSmem<S>>(kernel, blocks * p.segs, kBlock, stream, a, dm, seg_h, seg_d);
+    return launch_with<ForwardTeam, ForwardSmem<S, ForwardTeam>>(kernel, blocks * p.segs, stream, a, dm, seg_h, seg_d);
   });
 }
 
@@ -1043,7 +1117,7 @@ template <class T>
 cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaStream_t stream) {
   return by_slices(p.slices, [&](auto sc) -> cudaError_t {
     constexpr int S = decltype(sc)::value;
-    const ScanDims dm = scan_dims<T, S>(a, p);
+    const ScanDims dm = scan_dims<T, S, BackwardTeam>(a, p);
     const long long pieces = static_cast<long long>(p.row_chunks) * p.segs;
     const long long all = static_cast<long long>(a.dim) * a.state;
     const long long rows = static_cast<long long>(a.batch) * a.len * a.groups;
@@ -1055,12 +1129,13 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
     if (blocks * a.batch * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     cudaError_t e;
     if (p.segs > 1) {
-      e = launch_with<SegmentSmem<S>>(seq_scan_segment_kernel<T, S, true>, blocks * a.batch * (p.segs - 1),
-                                               kBlock, stream, a, dm, seg_h, seg_d);
+      const ScanDims dm = scan_dims<T, S, ForwardTeam>(a, p);
+      e = launch_with<ForwardTeam, SegmentSmem<S, ForwardTeam>>(seq_scan_segment_kernel<T, S, true>, blocks * a.batch * (p.segs - 1),
+                                               stream, a, dm, seg_h, seg_d);
       if (e != cudaSuccess) return e;
     }
     auto kernel = a.state == 4 * S ? seq_scan_bwd_kernel<T, S, false> : seq_scan_bwd_kernel<T, S, true>;
-    e = launch_with<BackwardSmem<S>>(kernel, blocks * pieces, kBlock, stream, a, dm, seg_h, seg_d,
+    e = launch_with<BackwardTeam, BackwardSmem<S, BackwardTeam>>(kernel, blocks * pieces, stream, a, dm, seg_h, seg_d,
                                         a.dB || a.dC ? part_bc : nullptr, part_p);
     if (e != cudaSuccess) return e;
     if (a.dB || a.dC) {
