@@ -22,7 +22,7 @@ cudaError_t scan_fwd(const pt_scan_args&, const ScanPlan&, float*, cudaStream_t)
 template <class T>
 cudaError_t scan_bwd(const pt_scan_args&, const ScanPlan&, float*, cudaStream_t);
 template <class T>
-cudaError_t scan_step(const pt_scan_args&, int, unsigned*, cudaStream_t);
+cudaError_t scan_step(const pt_scan_args&, int, int, unsigned*, cudaStream_t);
 
 namespace {
 
@@ -220,7 +220,7 @@ int pt_scan_step(const pt_scan_args* a, void* stream) {
   PT_TRY(seq_device(&sms, &err));
   const int slices = scan_plan(*a, sms, false).slices;
   return status(by_type(a->dtype, [&](auto t) {
-    return scan_step<decltype(t)>(*a, slices, err, static_cast<cudaStream_t>(stream));
+    return scan_step<decltype(t)>(*a, slices, sms, err, static_cast<cudaStream_t>(stream));
   }));
 }
 

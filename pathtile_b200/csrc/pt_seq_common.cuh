@@ -243,25 +243,17 @@ __device__ __forceinline__ void get_pairs(const float* src, F2 (&v)[(E + 1) / 2]
   }
 }
 
-// A row's state slot: -1 where there is none to touch.  Every thread of the
-// block calls it.  A slot at or past the cache's end (bit 7 of the device error
-// word) or one that an earlier row of the batch names too (bit 8) has none, so
-// no row writes outside the cache and no two rows write one state.
-__device__ __forceinline__ int slot_of(const int* __restrict__ slots, int row, int cache_rows, unsigned* err,
-                                       int thread, int threads) {
-  const int s = __ldg(slots + row);
-  if (s < 0) return -1;
-  if (s >= cache_rows) {
-    if (thread == 0) atomicOr(err, 128u);
-    return -1;
-  }
+// A row of a batch whose slot lies past the cache, or was named by an earlier row
+// too, is treated as padding and sets a bit of the device error word: no row
+// writes outside the cache, and no two rows write one state.
+constexpr unsigned kSlotPastCache = 1u << 7, kSlotTwice = 1u << 8;
+
+// Whether a row before `row` names the slot as well.  Every thread of the block calls it.
+__device__ __forceinline__ bool named_before(const int* __restrict__ slots, int row, int slot, int thread, int threads) {
   int twice = 0;
-  for (int i = thread; i < row; i += threads) twice |= __ldg(slots + i) == s;
-  if (__syncthreads_or(twice)) {
-    if (thread == 0) atomicOr(err, 256u);
-    return -1;
-  }
-  return s;
+  if (slot >= 0)
+    for (int i = thread; i < row; i += threads) twice |= __ldg(slots + i) == slot;
+  return __syncthreads_or(twice);
 }
 
 // Calls fn(T()) for the element type `dtype`.

@@ -345,12 +345,32 @@ __global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_arg
   const int cb = static_cast<int>(blockIdx.x) % cblocks, b = static_cast<int>(blockIdx.x) / cblocks;
   const int c = (cb * kConvThreads + static_cast<int>(threadIdx.x)) * V;
   const bool in = c < a.dim;
-  // What does not depend on the slot is under way while the slot is looked up.
+  const int tid = static_cast<int>(threadIdx.x);
+  int slot = a.slots ? __ldg(a.slots + b) : b;
+  if (slot >= a.cache_rows) {
+    if (tid == 0) atomicOr(err, kSlotPastCache);
+    slot = -1;
+  }
+  // Everything is on its way while the block looks whether an earlier row has the slot.
+  T* state = static_cast<T*>(a.state_out) + slot * a.state_row + c;
   Pack<T, V> win[K];
   Pack<float, V * K> w;
   Pack<float, V> bias;
   if (in) {
     win[K - 1].load(static_cast<const T*>(a.x) + b * a.x_batch + c, V, true);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+      // Plain loads, not the read-only ones: the cache is written below.
+      const T* p = state + static_cast<long long>(j) * a.dim;
+      if (slot < 0) {
+        win[j].zero();
+      } else if constexpr (V == 2 && sizeof(T) == 2) {
+        *reinterpret_cast<unsigned*>(win[j].v) = *reinterpret_cast<const unsigned*>(p);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[j].v[v] = p[v];
+      }
+    }
     if (a.param_f32) {
       w.load(static_cast<const float*>(a.w) + static_cast<long long>(c) * K, V * K, wide);
     } else {
@@ -360,7 +380,10 @@ __global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_arg
 #pragma unroll
     for (int v = 0; v < V; ++v) bias.v[v] = a.bias ? param<T>(a.bias, c + v, a.param_f32) : 0.f;
   }
-  const int slot = a.slots ? slot_of(a.slots, b, a.cache_rows, err, static_cast<int>(threadIdx.x), kConvThreads) : b;
+  if (a.slots && named_before(a.slots, b, slot, tid, kConvThreads)) {
+    if (tid == 0) atomicOr(err, kSlotTwice);
+    slot = -1;
+  }
   if (!in) return;
   T* y = static_cast<T*>(a.y) + static_cast<long long>(b) * a.dim + c;
   Pack<T, V> out;
@@ -368,18 +391,6 @@ __global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_arg
     out.zero();
     out.store(y, V, true);
     return;
-  }
-  T* state = static_cast<T*>(a.state_out) + static_cast<long long>(slot) * a.state_row + c;
-#pragma unroll
-  for (int j = 0; j < K - 1; ++j) {
-    // Plain loads, not the read-only ones: the cache is written below.
-    const T* p = state + static_cast<long long>(j) * a.dim;
-    if constexpr (V == 2 && sizeof(T) == 2) {
-      *reinterpret_cast<unsigned*>(win[j].v) = *reinterpret_cast<const unsigned*>(p);
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) win[j].v[v] = p[v];
-    }
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {

@@ -53,7 +53,10 @@ struct ScanTeam {
 // for 8 x 2048 x 2048 channels with 16 states in bf16; with four 243).  Backward,
 // four are enough and leave the scanners more registers (762 us; with eight, which
 // spill, 827).
-using ForwardTeam = ScanTeam<256, 112, 64>;
+// fp32 rows on their way take twice the registers (2048 x 48 x 256: 215 us, 283 us
+// with the other split).
+template <class T>
+using ForwardTeam = ScanTeam<256, sizeof(T) == 4 ? 80 : 112, sizeof(T) == 4 ? 80 : 64>;
 using BackwardTeam = ScanTeam<128, 136, 120>;
 
 template <int N>
@@ -290,9 +293,9 @@ struct SegmentSmem {
 };
 
 template <class T, int S, bool REV>
-__global__ void __launch_bounds__(ForwardTeam::kBlock, 2)
+__global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
     seq_scan_segment_kernel(pt_scan_args a, ScanDims dm, float* seg_h, float* seg_d) {
-  using TEAM = ForwardTeam;
+  using TEAM = ForwardTeam<T>;
   using P = ScanShape<S, TEAM>;
   extern __shared__ __align__(16) unsigned char smem[];
   auto& sm = *reinterpret_cast<SegmentSmem<S, TEAM>*>(smem);
@@ -427,9 +430,9 @@ struct ForwardSmem {
 };
 
 template <class T, int S, bool PAD>
-__global__ void __launch_bounds__(ForwardTeam::kBlock, 2)
+__global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
     seq_scan_fwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d) {
-  using TEAM = ForwardTeam;
+  using TEAM = ForwardTeam<T>;
   using P = ScanShape<S, TEAM>;
   extern __shared__ __align__(16) unsigned char smem[];
   auto& sm = *reinterpret_cast<ForwardSmem<S, TEAM>*>(smem);
@@ -987,57 +990,118 @@ __global__ void seq_scan_bc_kernel(const float* part, int cblocks, long long row
 }
 
 // ---------------------------------------------------------------- one token
-constexpr int kStepThreads = 128;
+// S lanes hold N neighbouring channels, each lane four states of every one.  The
+// first N lanes also take one channel each: its delta, its gate, its output;
+// what the others need of it crosses by shuffles, so nothing is computed twice.
+// Bound by reading and writing the states: those, and all else, are on their way
+// while the block looks whether an earlier row has the slot.
+template <int S>
+constexpr int kStepChannels = S == 2 ? 2 : 4;
 
-// A lane holds four states of a channel, S lanes the channel.
 template <class T, int S>
-__global__ void __launch_bounds__(kStepThreads) seq_scan_step_kernel(pt_scan_args a, int cblocks, bool wide,
-                                                                     unsigned* err) {
-  constexpr int kCh = kStepThreads / S;
+__global__ void __launch_bounds__(128) seq_scan_step_kernel(pt_scan_args a, int cblocks, int wide, unsigned* err) {
+  constexpr int N = kStepChannels<S>;
   const int cb = static_cast<int>(blockIdx.x) % cblocks, b = static_cast<int>(blockIdx.x) / cblocks;
-  const int tid = static_cast<int>(threadIdx.x);
-  const int slot = a.slots ? slot_of(a.slots, b, a.cache_rows, err, tid, kStepThreads) : b;
-  const int slice = tid & (S - 1), s0 = 4 * slice;
-  const int c = cb * kCh + tid / S;
-  const bool in = c < a.dim;
-  float y = 0.f;
-  if (in && slot >= 0) {
-    const int g = c / (a.dim / a.groups);
-    float d = to_f<T>(static_cast<const T*>(a.dt)[b * a.dt_batch + c]) + (a.dt_bias ? __ldg(a.dt_bias + c) : 0.f);
-    if (a.dt_softplus) d = softplusf(d);
-    const float v = d * to_f<T>(static_cast<const T*>(a.x)[b * a.x_batch + c]);
-    const T* Bp = static_cast<const T*>(a.B) + b * a.B_batch + g * a.B_group + s0;
-    const T* Cp = static_cast<const T*>(a.C) + b * a.C_batch + g * a.C_group + s0;
-    const float* Ap = a.A + static_cast<long long>(c) * a.state + s0;
-    float* hp = a.hlast + slot * a.h_row + static_cast<long long>(c) * a.state + s0;
-    if (wide && s0 + 4 <= a.state) {
-      float4 h = *reinterpret_cast<const float4*>(hp);
-      const float4 A = __ldg(reinterpret_cast<const float4*>(Ap));
-      h.x = fmaf(ex2(d * (A.x * kLog2e)), h.x, v * to_f<T>(Bp[0]));
-      h.y = fmaf(ex2(d * (A.y * kLog2e)), h.y, v * to_f<T>(Bp[1]));
-      h.z = fmaf(ex2(d * (A.z * kLog2e)), h.z, v * to_f<T>(Bp[2]));
-      h.w = fmaf(ex2(d * (A.w * kLog2e)), h.w, v * to_f<T>(Bp[3]));
-      y = fmaf(h.x, to_f<T>(Cp[0]), fmaf(h.y, to_f<T>(Cp[1]), fmaf(h.z, to_f<T>(Cp[2]), h.w * to_f<T>(Cp[3]))));
-      *reinterpret_cast<float4*>(hp) = h;
+  const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
+  const int slice = tid & (S - 1), s0 = 4 * slice, left = a.state - s0;  // left: states of this lane that exist
+  int slot = a.slots ? __ldg(a.slots + b) : b;
+  if (slot >= a.cache_rows) {
+    if (tid == 0) atomicOr(err, kSlotPastCache);
+    slot = -1;
+  }
+  const int c0 = (cb * (threads / S) + tid / S) * N;  // the lanes' first channel
+  const int n = min(N, a.dim - c0);                   // channels that exist
+  // B and C of the first channel's group; a group that begins within the N channels is rare.
+  int g = 0, next = a.dim;
+  if (a.groups > 1) {
+    const int per = a.dim / a.groups;
+    g = min(c0 / per, a.groups - 1), next = (g + 1) * per;
+  }
+  Pack<T, 4> B, C;
+  auto load_group = [&]() {
+    B.load(static_cast<const T*>(a.B) + b * a.B_batch + g * a.B_group + s0, left, wide & 2);
+    C.load(static_cast<const T*>(a.C) + b * a.C_batch + g * a.C_group + s0, left, wide & 2);
+  };
+  load_group();
+  float* hp = a.hlast + slot * a.h_row + static_cast<long long>(c0) * a.state + s0;
+  const float* Ap = a.A + static_cast<long long>(c0) * a.state + s0;
+  float h[N][4], A[N][4];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if ((wide & 1) && i < n && left > 0) {
+      const float4 Av = __ldg(reinterpret_cast<const float4*>(Ap + i * a.state));
+      A[i][0] = Av.x, A[i][1] = Av.y, A[i][2] = Av.z, A[i][3] = Av.w;
+      const float4 hv = slot >= 0 ? *reinterpret_cast<const float4*>(hp + i * a.state) : make_float4(0.f, 0.f, 0.f, 0.f);
+      h[i][0] = hv.x, h[i][1] = hv.y, h[i][2] = hv.z, h[i][3] = hv.w;
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (s0 + j < a.state) {
-          const float h = fmaf(ex2(d * (__ldg(Ap + j) * kLog2e)), hp[j], v * to_f<T>(Bp[j]));
-          y = fmaf(h, to_f<T>(Cp[j]), y);
-          hp[j] = h;
-        }
+        A[i][j] = i < n && j < left ? __ldg(Ap + i * a.state + j) : 0.f;
+        h[i][j] = i < n && j < left && slot >= 0 ? hp[i * a.state + j] : 0.f;
       }
     }
   }
+  // This lane's own channel.
+  const int c = c0 + slice;
+  const bool own = slice < n;
+  float delta = 0.f, v = 0.f, x = 0.f, z = 0.f, D = 0.f;
+  if (own) {
+    delta = to_f<T>(static_cast<const T*>(a.dt)[b * a.dt_batch + c]) + (a.dt_bias ? __ldg(a.dt_bias + c) : 0.f);
+    x = to_f<T>(static_cast<const T*>(a.x)[b * a.x_batch + c]);
+    if (a.z) z = to_f<T>(static_cast<const T*>(a.z)[b * a.z_batch + c]);
+    if (a.D) D = __ldg(a.D + c);
+    if (a.dt_softplus) delta = softplusf(delta);
+    v = delta * x;
+  }
+  if (a.slots && named_before(a.slots, b, slot, tid, threads)) {
+    if (tid == 0) atomicOr(err, kSlotTwice);
+    slot = -1;
+  }
+  float y[N];
 #pragma unroll
-  for (int m = 1; m < S; m *= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
-  if (in && slice == 0) {
-    if (slot >= 0) {
-      if (a.D) y = fmaf(__ldg(a.D + c), to_f<T>(static_cast<const T*>(a.x)[b * a.x_batch + c]), y);
-      if (a.z) y *= siluf(to_f<T>(static_cast<const T*>(a.z)[b * a.z_batch + c]));
+  for (int i = 0; i < N; ++i) {
+    const float d = __shfl_sync(0xffffffffu, delta, i, S) * kLog2e, u = __shfl_sync(0xffffffffu, v, i, S);
+    if (c0 + i >= next && i < n) {
+      ++g, next += a.dim / a.groups;
+      load_group();
     }
-    static_cast<T*>(a.y)[static_cast<long long>(b) * a.dim + c] = from_f<T>(y);
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) {
+        h[i][j] = fmaf(ex2(d * A[i][j]), h[i][j], u * B.f(j));
+        s = fmaf(h[i][j], C.f(j), s);
+      }
+    y[i] = s;
+    if (i < n && slot >= 0) {
+      if ((wide & 1) && left > 0) {
+        *reinterpret_cast<float4*>(hp + i * a.state) = make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j < left) hp[i * a.state + j] = h[i][j];
+      }
+    }
+  }
+  // Sums over the lanes; lane i < N ends with channel i's.
+  const bool odd = slice & 1;
+  if constexpr (N == 4) {
+    const bool up = slice & 2;
+    const float p = (up ? y[2] : y[0]) + __shfl_xor_sync(0xffffffffu, up ? y[0] : y[2], 2);
+    const float q = (up ? y[3] : y[1]) + __shfl_xor_sync(0xffffffffu, up ? y[1] : y[3], 2);
+    y[0] = p, y[1] = q;
+  }
+  float sum = (odd ? y[1] : y[0]) + __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[1], 1);
+#pragma unroll
+  for (int m = 4; m < S; m *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+  if (own) {
+    if (slot >= 0) {
+      if (a.D) sum = fmaf(D, x, sum);
+      if (a.z) sum *= siluf(z);
+    } else {
+      sum = 0.f;
+    }
+    static_cast<T*>(a.y)[static_cast<long long>(b) * a.dim + c] = from_f<T>(sum);
   }
 }
 
@@ -1098,18 +1162,18 @@ template <class T>
 cudaError_t scan_fwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaStream_t stream) {
   return by_slices(p.slices, [&](auto sc) -> cudaError_t {
     constexpr int S = decltype(sc)::value;
-    const ScanDims dm = scan_dims<T, S, ForwardTeam>(a, p);
+    const ScanDims dm = scan_dims<T, S, ForwardTeam<T>>(a, p);
     float* seg_h = ws;
     float* seg_d = ws + static_cast<size_t>(a.batch) * p.segs * a.dim * a.state;
     const long long blocks = static_cast<long long>(p.cblocks) * a.groups * a.batch;
     if (blocks * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     if (p.segs > 1) {
-      const cudaError_t e = launch_with<ForwardTeam, SegmentSmem<S, ForwardTeam>>(
+      const cudaError_t e = launch_with<ForwardTeam<T>, SegmentSmem<S, ForwardTeam<T>>>(
           seq_scan_segment_kernel<T, S, false>, blocks * (p.segs - 1), stream, a, dm, seg_h, seg_d);
       if (e != cudaSuccess) return e;
     }
     auto kernel = a.state == 4 * S ? seq_scan_fwd_kernel<T, S, false> : seq_scan_fwd_kernel<T, S, true>;
-    return launch_with<ForwardTeam, ForwardSmem<S, ForwardTeam>>(kernel, blocks * p.segs, stream, a, dm, seg_h, seg_d);
+    return launch_with<ForwardTeam<T>, ForwardSmem<S, ForwardTeam<T>>>(kernel, blocks * p.segs, stream, a, dm, seg_h, seg_d);
   });
 }
 
@@ -1129,8 +1193,8 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
     if (blocks * a.batch * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     cudaError_t e;
     if (p.segs > 1) {
-      const ScanDims dm = scan_dims<T, S, ForwardTeam>(a, p);
-      e = launch_with<ForwardTeam, SegmentSmem<S, ForwardTeam>>(seq_scan_segment_kernel<T, S, true>, blocks * a.batch * (p.segs - 1),
+      const ScanDims dm = scan_dims<T, S, ForwardTeam<T>>(a, p);
+      e = launch_with<ForwardTeam<T>, SegmentSmem<S, ForwardTeam<T>>>(seq_scan_segment_kernel<T, S, true>, blocks * a.batch * (p.segs - 1),
                                                stream, a, dm, seg_h, seg_d);
       if (e != cudaSuccess) return e;
     }
@@ -1152,14 +1216,23 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
 }
 
 template <class T>
-cudaError_t scan_step(const pt_scan_args& a, int slices, unsigned* err, cudaStream_t stream) {
+cudaError_t scan_step(const pt_scan_args& a, int slices, int sm_count, unsigned* err, cudaStream_t stream) {
   return by_slices(slices, [&](auto sc) -> cudaError_t {
     constexpr int S = decltype(sc)::value;
-    const int cblocks = static_cast<int>(cdiv(a.dim, kStepThreads / S));
+    const long long lanes = cdiv(a.dim, kStepChannels<S>) * S;
+    // A call that does not fill the SMs is spread over small blocks.
+    const int threads = lanes * a.batch < 512LL * sm_count ? 32 : 128;
+    const int cblocks = static_cast<int>(cdiv(lanes, threads));
     const long long grid = static_cast<long long>(cblocks) * a.batch;
     if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-    const bool wide = a.state % 4 == 0 && a.h_row % 4 == 0 && aligned(a.hlast, 16) && aligned(a.A, 16);
-    seq_scan_step_kernel<T, S><<<static_cast<unsigned>(grid), kStepThreads, 0, stream>>>(a, cblocks, wide, err);
+    // Bit 0: states and rates, bit 1: B and C move four at a time.
+    const size_t four = 4 * sizeof(T);
+    int wide = a.state % 4 == 0 && a.h_row % 4 == 0 && aligned(a.hlast, 16) && aligned(a.A, 16);
+    wide |= a.state % 4 == 0 && aligned(a.B, four) && aligned(a.C, four) && a.B_batch % 4 == 0 && a.B_group % 4 == 0 &&
+                    a.C_batch % 4 == 0 && a.C_group % 4 == 0
+                ? 2
+                : 0;
+    seq_scan_step_kernel<T, S><<<static_cast<unsigned>(grid), threads, 0, stream>>>(a, cblocks, wide, err);
     return cudaGetLastError();
   });
 }

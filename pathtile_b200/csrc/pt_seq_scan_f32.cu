@@ -5,6 +5,6 @@ namespace pt {
 namespace seq {
 template cudaError_t scan_fwd<float>(const pt_scan_args&, const ScanPlan&, float*, cudaStream_t);
 template cudaError_t scan_bwd<float>(const pt_scan_args&, const ScanPlan&, float*, cudaStream_t);
-template cudaError_t scan_step<float>(const pt_scan_args&, int, unsigned*, cudaStream_t);
+template cudaError_t scan_step<float>(const pt_scan_args&, int, int, unsigned*, cudaStream_t);
 }  // namespace seq
 }  // namespace pt
