@@ -258,9 +258,16 @@ __device__ __forceinline__ void put_sums(float (*dst)[64 / S * kScanWarps], int 
   }
 }
 
+// How the states fill their lanes' fours: all do, some lanes have none, or one
+// lane has some.  What padded states hold must not reach a sum (0 x inf): a lane
+// without states gives 0, a lane with some leaves the others out one by one.
+enum Fill { kFull, kLanes, kPartial };
+inline Fill fill_of(int states, int slices) {
+  return states == 4 * slices ? kFull : states % 4 == 0 ? kLanes : kPartial;
+}
+
 // s + h . c over the pair's states that exist.
 __device__ __forceinline__ float dot2(F2 h, F2 c, float s, int first, int states) {
-  // States past the last one are not the operator's: 0 x inf must not reach the sum.
   if (first < states) s = fmaf(lo2(h), lo2(c), s);
   if (first + 1 < states) s = fmaf(hi2(h), hi2(c), s);
   return s;
@@ -429,7 +436,7 @@ struct ForwardSmem {
   float B[2][kTile][P::kStates], C[2][kTile][P::kStates];
 };
 
-template <class T, int S, bool PAD>
+template <class T, int S, Fill FILL>
 __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
     seq_scan_fwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d) {
   using TEAM = ForwardTeam<T>;
@@ -584,11 +591,12 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
           for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int p = 0; p < 2; ++p) h[c][p] = fma2(e[q][c][p], h[c][p], mul2(v[q].v[c], B[q].v[p]));
-            if constexpr (PAD) {
+            if constexpr (FILL == kPartial) {
               y[q][c] = dot2(h[c][1], C[q].v[1], dot2(h[c][0], C[q].v[0], 0.f, me.s0, a.state), me.s0 + 2, a.state);
             } else {
               const F2 s = fma2(h[c][1], C[q].v[1], mul2(h[c][0], C[q].v[0]));
               y[q][c] = lo2(s) + hi2(s);
+              if (FILL == kLanes && me.s0 >= a.state) y[q][c] = 0.f;
             }
           }
         if (i > 0) {
@@ -665,7 +673,7 @@ struct BackwardSmem {
   float accD[kTile][P::kCh], accb[kTile][P::kCh];     // dD and ddt_bias at the end
 };
 
-template <class T, int S, bool PAD>
+template <class T, int S, Fill FILL>
 __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
     seq_scan_bwd_kernel(pt_scan_args a, ScanDims dm, const float* seg_h, const float* seg_d, float* part_bc,
                         float* part_p) {
@@ -920,7 +928,7 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
               g[c][p] = mul2(as[i][c][p], dh);
               const F2 dlog = mul2(g[c][p], hs[i][c][p]);
               dA[c][p] = fma2(dlog, d.v[c], dA[c][p]);
-              if constexpr (PAD) {
+              if constexpr (FILL == kPartial) {
                 const int f = me.s0 + 2 * p;
                 sB = pack2(dot2(dh, B.v[p], lo2(sB), f, a.state), 0.f);
                 sA = pack2(dot2(dlog, A2[c][p], lo2(sA), f, a.state), 0.f);
@@ -934,6 +942,7 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
             gB[i & 1][c] = lo2(sB) + hi2(sB);
             gA[i & 1][c] = lo2(sA) + hi2(sA);
             yy[i & 1][c] = lo2(sy) + hi2(sy);
+            if (FILL == kLanes && me.s0 >= a.state) gB[i & 1][c] = gA[i & 1][c] = yy[i & 1][c] = 0.f;
           }
           float bc[8] = {lo2(bB[0]), hi2(bB[0]), lo2(bB[1]), hi2(bB[1]), lo2(bC[0]), hi2(bC[0]), lo2(bC[1]), hi2(bC[1])};
           sum_channels<S>(bc, me.lane, sm.red[st][me.warp][i0 + i]);
@@ -1172,7 +1181,10 @@ cudaError_t scan_fwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
           seq_scan_segment_kernel<T, S, false>, blocks * (p.segs - 1), stream, a, dm, seg_h, seg_d);
       if (e != cudaSuccess) return e;
     }
-    auto kernel = a.state == 4 * S ? seq_scan_fwd_kernel<T, S, false> : seq_scan_fwd_kernel<T, S, true>;
+    const Fill fill = fill_of(a.state, S);
+    auto kernel = fill == kFull    ? seq_scan_fwd_kernel<T, S, kFull>
+                  : fill == kLanes ? seq_scan_fwd_kernel<T, S, kLanes>
+                                   : seq_scan_fwd_kernel<T, S, kPartial>;
     return launch_with<ForwardTeam<T>, ForwardSmem<S, ForwardTeam<T>>>(kernel, blocks * p.segs, stream, a, dm, seg_h, seg_d);
   });
 }
@@ -1198,7 +1210,10 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
                                                stream, a, dm, seg_h, seg_d);
       if (e != cudaSuccess) return e;
     }
-    auto kernel = a.state == 4 * S ? seq_scan_bwd_kernel<T, S, false> : seq_scan_bwd_kernel<T, S, true>;
+    const Fill fill = fill_of(a.state, S);
+    auto kernel = fill == kFull    ? seq_scan_bwd_kernel<T, S, kFull>
+                  : fill == kLanes ? seq_scan_bwd_kernel<T, S, kLanes>
+                                   : seq_scan_bwd_kernel<T, S, kPartial>;
     e = launch_with<BackwardTeam, BackwardSmem<S, BackwardTeam>>(kernel, blocks * pieces, stream, a, dm, seg_h, seg_d,
                                         a.dB || a.dC ? part_bc : nullptr, part_p);
     if (e != cudaSuccess) return e;
