@@ -165,35 +165,48 @@ __global__ void __launch_bounds__(kConvThreads, kConvFwdBlocks<V>)
       win[j + 1].from(p);
     }
     T* y = static_cast<T*>(a.y) + at * a.dim + c;
-    Pack<T, V> next[U];
+    const T* x = row.x + t0 * row.step;
+    auto advance = [&](const Pack<T, V>& in) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) row.load(next[u], t0 + u);
-    for (int t = t0; t < t1; t += U) {
+      for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
+      win[K - 1].from(in);
+      Packed<V> s;
+#pragma unroll
+      for (int i = 0; i < Packed<V>::N; ++i) {
+        s.p[i] = taps.pre(win, i);
+        if (a.silu) s.p[i] = mul2(s.p[i], sigmoid2(s.p[i]));
+      }
+      Pack<T, V> out;
+      s.to(out);
+      out.store(y, V, true);
+      y += a.dim;
+    };
+    // U steps at a time, the next ones on their way; the rest one by one; zeros behind the row's end.
+    int t = t0;
+    const int valid = min(t1, row.len);
+    Pack<T, V> next[U];
+    auto fetch = [&]() {
+#pragma unroll
+      for (int u = 0; u < U; ++u, x += row.step) next[u].load(x, V, true);
+    };
+    if (t + U <= valid) fetch();
+    for (; t + U <= valid; t += U) {
       Pack<T, V> in[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) in[u] = next[u];
-      if (t + U < t1) {
+      if (t + 2 * U <= valid) fetch();
 #pragma unroll
-        for (int u = 0; u < U; ++u) row.load(next[u], t + U + u);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
-        win[K - 1].from(in[u]);
-        Packed<V> s;
-#pragma unroll
-        for (int i = 0; i < Packed<V>::N; ++i) {
-          s.p[i] = taps.pre(win, i);
-          if (a.silu) s.p[i] = mul2(s.p[i], sigmoid2(s.p[i]));
-        }
-        if (t + u < t1) {
-          Pack<T, V> out;
-          s.to(out);
-          if (t + u >= row.len) out.zero();
-          out.store(y + static_cast<long long>(t + u - t0) * a.dim, V, true);
-        }
-      }
+      for (int u = 0; u < U; ++u) advance(in[u]);
+    }
+    for (; t < valid; ++t, x += row.step) {
+      Pack<T, V> in;
+      in.load(x, V, true);
+      advance(in);
+    }
+    for (; t < t1; ++t, y += a.dim) {
+      Pack<T, V> out;
+      out.zero();
+      out.store(y, V, true);
     }
     at += t1 - t0;
   }
@@ -222,70 +235,84 @@ __device__ __forceinline__ void conv_bwd_stretch(const pt_conv_args& a, const Ta
     win[j + 1].from(p);
   }
   const int first = t0 == 0 ? -(K - 1) : t0;  // first position whose gradient is written here
-  auto load_dy = [&](Pack<T, V>& p, int t) {
-    if (t < len)
-      p.load(dy + t * a.dy_step, V, true);
-    else
-      p.zero();
-  };
-  Pack<T, V> xn[U], gn[U];
+  const T* x = row.x + t0 * row.step;
+  dy += t0 * a.dy_step;
+  if (dx) dx += static_cast<long long>(t0 - (K - 1)) * a.dim;  // moves on with t, to position t - K + 1
+  // Step t.  In the middle of a row (INNER) the step is valid and its position's gradient is this thread's to write;
+  // elsewhere each of that is asked for.
+  auto advance = [&](const Pack<T, V>& xin, const Pack<T, V>& gin, int t, auto inner) {
+    constexpr bool INNER = decltype(inner)::value;
+    const int pos = t - (K - 1);
+    Packed<V> g, s;
+    g.from(gin);
 #pragma unroll
-  for (int u = 0; u < U; ++u) row.load(xn[u], t0 + u), load_dy(gn[u], t0 + u);
-  for (int tt = t0; tt < t1 + K - 1; tt += U) {
+    for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
+    win[K - 1].from(xin);
+#pragma unroll
+    for (int i = 0; i < Packed<V>::N; ++i) {
+      if (a.silu) {
+        const F2 pre = taps.pre(win, i), sig = sigmoid2(pre);
+        g.p[i] = mul2(g.p[i], silu_grad2(pre, sig));
+      }
+      // Steps behind the row's end have no output; their window may hold anything.
+      if (!INNER && t >= len) g.p[i] = 0;
+      if (INNER || (t < t1 && t < len)) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) dw[j].p[i] = fma2(g.p[i], win[j].p[i], dw[j].p[i]);
+        db.p[i] = add2(db.p[i], g.p[i]);
+      }
+#pragma unroll
+      for (int j = K - 1; j > 0; --j) gw[j].p[i] = gw[j - 1].p[i];
+      gw[0].p[i] = g.p[i];
+      s.p[i] = 0;
+#pragma unroll
+      for (int j = 0; j < K; ++j) s.p[i] = fma2(taps.w[j].p[i], gw[j].p[i], s.p[i]);
+    }
+    if (INNER || (pos >= first && pos < t1)) {
+      if (!INNER && dso && pos >= len - (K - 1) && pos < len) {
+        Pack<T, V> more;
+        more.load(dso + static_cast<long long>(pos - (len - (K - 1))) * a.dim, V, true);
+#pragma unroll
+        for (int i = 0; i < Packed<V>::N; ++i) s.p[i] = add2(s.p[i], more.pair(i));
+      }
+      Pack<T, V> out;
+      s.to(out);
+      if (INNER || pos >= 0) {
+        if (dx) out.store(dx, V, true);
+      } else if (dsi) {
+        out.store(dsi + static_cast<long long>(pos + K - 1) * a.dim, V, true);
+      }
+    }
+    if (dx) dx += a.dim;
+  };
+  auto edge = [&](int t) {
+    Pack<T, V> xin, gin;
+    if (t < len) {
+      xin.load(x, V, true), gin.load(dy, V, true);
+    } else {
+      xin.zero(), gin.zero();
+    }
+    x += row.step, dy += a.dy_step;
+    advance(xin, gin, t, std::integral_constant<bool, false>());
+  };
+  int t = t0;
+  const int end = t1 + K - 1, valid = min(t1, len);
+  for (; t < t0 + K - 1 && t < end; ++t) edge(t);
+  Pack<T, V> xn[U], gn[U];
+  auto fetch = [&]() {
+#pragma unroll
+    for (int u = 0; u < U; ++u, x += row.step, dy += a.dy_step) xn[u].load(x, V, true), gn[u].load(dy, V, true);
+  };
+  if (t + U <= valid) fetch();
+  for (; t + U <= valid; t += U) {
     Pack<T, V> xin[U], gin[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) xin[u] = xn[u], gin[u] = gn[u];
-    if (tt + U < t1 + K - 1) {
+    if (t + 2 * U <= valid) fetch();
 #pragma unroll
-      for (int u = 0; u < U; ++u) row.load(xn[u], tt + U + u), load_dy(gn[u], tt + U + u);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = tt + u, pos = t - (K - 1);
-      Packed<V> g, s;
-      g.from(gin[u]);
-#pragma unroll
-      for (int j = 0; j < K - 1; ++j) win[j] = win[j + 1];
-      win[K - 1].from(xin[u]);
-#pragma unroll
-      for (int i = 0; i < Packed<V>::N; ++i) {
-        if (a.silu) {
-          const F2 pre = taps.pre(win, i), sig = sigmoid2(pre);
-          g.p[i] = mul2(g.p[i], silu_grad2(pre, sig));
-        }
-        // Steps behind the row's end have no output; their window may hold anything.
-        if (t >= len) g.p[i] = 0;
-        if (t < t1 && t < len) {
-#pragma unroll
-          for (int j = 0; j < K; ++j) dw[j].p[i] = fma2(g.p[i], win[j].p[i], dw[j].p[i]);
-          db.p[i] = add2(db.p[i], g.p[i]);
-        }
-#pragma unroll
-        for (int j = K - 1; j > 0; --j) gw[j].p[i] = gw[j - 1].p[i];
-        gw[0].p[i] = g.p[i];
-        s.p[i] = 0;
-#pragma unroll
-        for (int j = 0; j < K; ++j) s.p[i] = fma2(taps.w[j].p[i], gw[j].p[i], s.p[i]);
-      }
-      if (pos >= first && pos < t1) {
-        if (dso && pos >= len - (K - 1) && pos < len) {
-          Pack<T, V> more;
-          more.load(dso + static_cast<long long>(pos - (len - (K - 1))) * a.dim, V, true);
-          Packed<V> m;
-          m.from(more);
-#pragma unroll
-          for (int i = 0; i < Packed<V>::N; ++i) s.p[i] = add2(s.p[i], m.p[i]);
-        }
-        Pack<T, V> out;
-        s.to(out);
-        if (pos >= 0) {
-          if (dx) out.store(dx + static_cast<long long>(pos) * a.dim, V, true);
-        } else if (dsi) {
-          out.store(dsi + static_cast<long long>(pos + K - 1) * a.dim, V, true);
-        }
-      }
-    }
+    for (int u = 0; u < U; ++u) advance(xin[u], gin[u], t + u, std::integral_constant<bool, true>());
   }
+  for (; t < end; ++t) edge(t);
 }
 
 template <class T, int K, int V>
@@ -491,7 +518,9 @@ ConvBwdPlan conv_bwd_plan(const pt_conv_args& a, int sm_count) {
 template <class T>
 cudaError_t conv_fwd(const pt_conv_args& a, int sm_count, cudaStream_t stream) {
   const int v = conv_width(a, sizeof(T), conv_word<T>);
-  const ConvCut p = conv_cut(a, v, (v > 2 ? kConvFwdBlocks<4> : kConvFwdBlocks<2>) * static_cast<long long>(kConvThreads) * sm_count, 8);
+  // One wave; with rows of different lengths four, whose stretches are dealt out as blocks finish.
+  const int blocks = (v > 2 ? kConvFwdBlocks<4> : kConvFwdBlocks<2>) * (a.lengths ? 4 : 1);
+  const ConvCut p = conv_cut(a, v, static_cast<long long>(blocks) * kConvThreads * sm_count, 8);
   const long long grid = p.cblocks * cdiv(p.walkers, p.ty);
   if (grid > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   return by_width_taps<conv_word<T>>(v, a.taps, [&](auto vc, auto kc) {
