@@ -7,7 +7,7 @@ K <= 48, behind the operator API of the reference's kernels/warp_tiled.py
 ``libpathtile_b200.so`` (C ABI: include/pathtile_b200.h); there is no host
 fallback.  :mod:`pathtile_b200.sequence` adds the operators of a selective
 state space block: causal convolution, selective scan and fused norm, with
-their single-token forms.
+their single-token forms; :mod:`pathtile_b200.selective` is the block.
 """
 from ._lib import PathTileError
 from .ops import dk, dx, fwd

@@ -22,6 +22,10 @@ Two B200-side changes, neither of which changes the function computed:
 convolution; a conv function with a true ``channels_last`` attribute gets
 [B, L, H] tensors, any other gets [B, H, L] (the reference's layout).  By
 default every block uses the native channels-last operator.
+
+``Model(block="selective")`` puts selective state space blocks
+(:mod:`pathtile_b200.selective`) in the S4 blocks' place; the training loop is
+the same.  There is no counterpart in the reference.
 """
 from __future__ import annotations
 
@@ -34,6 +38,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .runtime import MAX_L, depthwise_conv_b200_cl
+from .selective import SelectiveBlock
+from .sequence import fused_norm
 
 ConvFn = Callable[[torch.Tensor, torch.Tensor], torch.Tensor]
 
@@ -109,17 +115,34 @@ class S4ConvBlock(nn.Module):
 
 
 class Model(nn.Module):
-    """Encoder -> S4 blocks -> decoder; input [B, L, input_dim], output [B, output_dim]."""
+    """Encoder -> blocks -> decoder; input [B, L, input_dim], output [B, output_dim].
+
+    ``block``: "s4", or "selective" for selective state space blocks, whose
+    ``state_dim`` is up to 64 and which take any L (dropout and conv are the S4
+    blocks')."""
 
     def __init__(self, state_dim: int = 64, hidden_dim: int = 128, input_dim: int = 4, output_dim: int = 1,
-                 num_blocks: int = 4, dropout: float = 0.01, conv: ConvFn = depthwise_conv_b200_cl) -> None:
+                 num_blocks: int = 4, dropout: float = 0.01, conv: ConvFn = depthwise_conv_b200_cl,
+                 block: str = "s4") -> None:
         super().__init__()
+        if block not in ("s4", "selective"):
+            raise ValueError(f'block must be "s4" or "selective", got {block!r}')
         self.encoder = nn.Linear(input_dim, hidden_dim)
-        self.blocks = nn.ModuleList([S4ConvBlock(hidden_dim, state_dim, dropout, conv) for _ in range(num_blocks)])
+        self.selective = block == "selective"
+        self.blocks = nn.ModuleList([SelectiveBlock(hidden_dim, state_dim) if self.selective
+                                     else S4ConvBlock(hidden_dim, state_dim, dropout, conv) for _ in range(num_blocks)])
+        if self.selective:
+            self.norm_weight = nn.Parameter(torch.ones(hidden_dim))
         self.decoder = nn.Linear(hidden_dim, output_dim)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x = self.encoder(x)
+        if self.selective:
+            residual = None
+            for block in self.blocks:
+                x, residual = block(x, residual)
+            x = fused_norm(x, self.norm_weight, residual=residual)[0] if residual is not None else x
+            return self.decoder(x[:, -1, :])
         for block in self.blocks:
             x = block(x)
         return self.decoder(x)[:, -1, :]

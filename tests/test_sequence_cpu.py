@@ -249,3 +249,17 @@ def test_norm_definition_against_autograd(parts):
     torch.testing.assert_close(got["y"], y.detach())
     for name, grad in zip(named, grads):
         torch.testing.assert_close(got["d" + name], grad, msg=name)
+
+
+# ---------------------------------------------------------------- the block that calls them
+def test_the_model_offers_both_blocks():
+    from pathtile_b200 import s4conv, selective
+
+    plain = s4conv.Model(hidden_dim=16, num_blocks=1)
+    assert not any("norm" in n for n in plain.state_dict())  # the S4 model's state dict is as it was
+    model = s4conv.Model(hidden_dim=16, state_dim=8, num_blocks=2, block="selective")
+    assert all(isinstance(b, selective.SelectiveBlock) for b in model.blocks)
+    cache = model.blocks[0].make_cache(3)
+    assert cache.window.shape == (3, 3, 32) and cache.state.shape == (3, 32, 8)
+    with pytest.raises(ValueError, match="block"):
+        s4conv.Model(block="other")
