@@ -208,6 +208,14 @@ __device__ __forceinline__ void load_rates(const pt_scan_args& a, const Scanner<
     for (int p = 0; p < 2; ++p) A2[i][p] = mul2(A2[i][p], pack2(kLog2e, kLog2e));
 }
 
+// exp(delta A) = 2^(delta A2).  A state that forgets slowly multiplies hundreds of
+// these, so what counts is their mean error: the hardware's 2^x lies 2e-8 low on
+// the average between -0.25 and -0.001 (measured; a float's half step below 1 is
+// 3e-8).  Raising the exponent by 2e-8 costs nothing and leaves a few 1e-9; 2^0
+// stays 1, so a step of no duration leaves a state as it is.
+constexpr float kCentre = 2e-8f;
+__device__ __forceinline__ F2 decay(F2 delta, F2 A2) { return ex2x2(fma2(delta, A2, same2(kCentre))); }
+
 // A channel pair's values of one step, each twice: ready for packed arithmetic over states.
 struct Both {
   F2 v[2];
@@ -397,7 +405,7 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
         dsum[c] += lo2(d.v[c]);
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const F2 e = ex2x2(mul2(d.v[c], A2[c][p]));
+          const F2 e = decay(d.v[c], A2[c][p]);
           h[c][p] = REV ? mul2(e, fma2(v.v[c], B.v[p], h[c][p])) : fma2(e, h[c][p], mul2(v.v[c], B.v[p]));
         }
       }
@@ -424,7 +432,7 @@ __device__ __forceinline__ void join_segment(const pt_scan_args& a, const ScanDi
   for (int i = 0; i < 2; ++i) {
     const float d = i < me.mine ? seg_d[row * a.dim + me.c + i] : 0.f;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) h[i][p] = fma2(ex2x2(mul2(pack2(d, d), A2[i][p])), h[i][p], l[i][p]);
+    for (int p = 0; p < 2; ++p) h[i][p] = fma2(decay(pack2(d, d), A2[i][p]), h[i][p], l[i][p]);
   }
 }
 
@@ -561,7 +569,7 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int p = 0; p < 2; ++p) e[q][c][p] = ex2x2(mul2(dn[q].v[c], A2[c][p]));
+          for (int p = 0; p < 2; ++p) e[q][c][p] = decay(dn[q].v[c], A2[c][p]);
       dn[0] = Both(&sm.d[st][2][me.cl]), dn[1] = Both(&sm.d[st][3][me.cl]);
       float last[2][2];
 #pragma unroll
@@ -576,7 +584,7 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int p = 0; p < 2; ++p) en[q][c][p] = ex2x2(mul2(dn[q].v[c], A2[c][p]));
+              for (int p = 0; p < 2; ++p) en[q][c][p] = decay(dn[q].v[c], A2[c][p]);
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             vn[q] = Both(&sm.v[st][i + 2 + q][me.cl]);
@@ -879,7 +887,7 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int p = 0; p < 2; ++p)
-              h[c][p] = fma2(ex2x2(mul2(d.v[c], A2[c][p])), h[c][p], mul2(v.v[c], B.v[p]));
+              h[c][p] = fma2(decay(d.v[c], A2[c][p]), h[c][p], mul2(v.v[c], B.v[p]));
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -907,7 +915,7 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-              as[i][c][p] = ex2x2(mul2(d.v[c], A2[c][p]));
+              as[i][c][p] = decay(d.v[c], A2[c][p]);
               hs[i + 1][c][p] = fma2(as[i][c][p], hs[i][c][p], mul2(v.v[c], B.v[p]));
             }
         }
@@ -1078,7 +1086,7 @@ __global__ void __launch_bounds__(128) seq_scan_step_kernel(pt_scan_args a, int 
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (j < left) {
-        h[i][j] = fmaf(ex2(d * A[i][j]), h[i][j], u * B.f(j));
+        h[i][j] = fmaf(ex2(fmaf(d, A[i][j], kCentre)), h[i][j], u * B.f(j));
         s = fmaf(h[i][j], C.f(j), s);
       }
     y[i] = s;

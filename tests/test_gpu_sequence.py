@@ -265,6 +265,22 @@ def test_selective_scan_step_continues_a_prompt(cuda_device, b, d, n, g, dtype):
     close(state, one["state"], size["state"], 4 * 6 + n + 32, "state")
 
 
+def test_steps_behind_a_rows_end_leave_its_state_as_it_is(cuda_device):
+    """Bit for bit, over thousands of them: the state of a padded row is that of the row alone (from zero: a long
+    call joins pieces, and adds an initial state in another order), and an empty row's the initial one."""
+    m = Maker(cuda_device, 26)
+    for length, used in ((4000, 3), (4000, 0), (70, 33), (20, 7), (20, 0)):
+        v = scan_inputs(m, 1, length, 16, 16, 1, F32, True, True, True, used == 0, False)
+        v["A"][0] = 0.0
+        lengths = torch.tensor([used], dtype=torch.int32, device=cuda_device)
+        _, padded = pt.selective_scan(**v, dt_softplus=True, return_final_state=True, lengths=lengths)
+        short = {k: t[:, :used] if k in ("x", "dt", "B", "C", "z") else t for k, t in v.items()}
+        _, alone = pt.selective_scan(**short, dt_softplus=True, return_final_state=True)
+        assert torch.equal(padded, alone)
+        if used == 0:
+            assert torch.equal(padded, v["initial_state"])
+
+
 # ---------------------------------------------------------------- slots
 def _step_both(device, slots, rows, d=40, n=16, k=4):
     """Both step forms with these slots; returns (cache before, cache after, y, row b's y were it alone) for each."""
