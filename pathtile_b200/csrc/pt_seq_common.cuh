@@ -173,6 +173,7 @@ __device__ __forceinline__ float silu_grad(float v, float s) { return s * fmaf(v
 
 __device__ __forceinline__ F2 ex2x2(F2 x) { return pack2(ex2(lo2(x)), ex2(hi2(x))); }
 __device__ __forceinline__ F2 same2(float v) { return pack2(v, v); }
+__device__ __forceinline__ float sum2(F2 v) { return lo2(v) + hi2(v); }
 __device__ __forceinline__ F2 rcp2(F2 v) { return pack2(rcp(lo2(v)), rcp(hi2(v))); }
 __device__ __forceinline__ F2 sigmoid2(F2 v) {
   return rcp2(add2(ex2x2(mul2(v, same2(-kLog2e))), same2(1.f)));

@@ -25,26 +25,80 @@ namespace {
 // other combination runs the general one.
 enum NormForm { kGated, kResidual, kAny };
 
-// V parameters from index i on (zeros from no pointer).
-template <class T, int V>
-__device__ __forceinline__ void load_param(const void* p, int i, int n, bool f32, float (&out)[V]) {
-  if (!p) {
+// What a thread holds of a row: NV words of V elements, `threads` words apart, as
+// packed pairs (neighbours in a word; of single elements, two words' together).
+// Words past the row's end are zeros.
+template <int V, int NV>
+struct Words {
+  static_assert(V * NV % 2 == 0, "whole pairs");
+  static constexpr int N = V * NV / 2;
+
+  template <class T>
+  static __device__ __forceinline__ void load(Pack<T, V> (&w)[NV], const T* row, int width) {
+    const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
 #pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = 0.f;
-    return;
+    for (int k = 0; k < NV; ++k) {
+      const int i = (k * threads + tid) * V;
+      if (i < width)
+        w[k].load(row + i, V, true);
+      else
+        w[k].zero();
+    }
   }
-  if (f32) {
-    Pack<float, V> w;
-    w.load(static_cast<const float*>(p) + i, n, true);
+  template <class T>
+  static __device__ __forceinline__ void store(const Pack<T, V> (&w)[NV], T* row, int width) {
+    const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
 #pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = w.f(v);
-  } else {
-    Pack<T, V> w;
-    w.load(static_cast<const T*>(p) + i, n, true);
-#pragma unroll
-    for (int v = 0; v < V; ++v) out[v] = w.f(v);
+    for (int k = 0; k < NV; ++k) {
+      const int i = (k * threads + tid) * V;
+      if (i < width) w[k].store(row + i, V, true);
+    }
   }
-}
+  template <class T>
+  static __device__ __forceinline__ F2 get(const Pack<T, V> (&w)[NV], int q) {
+    if constexpr (V > 1)
+      return w[q / (V / 2)].pair(q % (V / 2));
+    else
+      return pack2(w[2 * q].f(0), w[2 * q + 1].f(0));
+  }
+  template <class T>
+  static __device__ __forceinline__ void set(Pack<T, V> (&w)[NV], int q, F2 v) {
+    if constexpr (V > 1)
+      w[q / (V / 2)].set_pair(q % (V / 2), v);
+    else
+      w[2 * q].set(0, lo2(v)), w[2 * q + 1].set(0, hi2(v));
+  }
+  // Parameters in fp32 or the activations' type; zeros from no pointer.
+  template <class T>
+  static __device__ __forceinline__ void params(const void* p, int first, int width, bool f32, F2 (&out)[N]) {
+    if (!p) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) out[q] = 0;
+    } else if (f32) {
+      Pack<float, V> w[NV];
+      load(w, static_cast<const float*>(p) + first, width);
+#pragma unroll
+      for (int q = 0; q < N; ++q) out[q] = get(w, q);
+    } else {
+      Pack<T, V> w[NV];
+      load(w, static_cast<const T*>(p) + first, width);
+#pragma unroll
+      for (int q = 0; q < N; ++q) out[q] = get(w, q);
+    }
+  }
+  // fp32, one row of a partial sum.
+  static __device__ __forceinline__ void put(const F2 (&v)[N], float* row, int width) {
+    Pack<float, V> w[NV];
+#pragma unroll
+    for (int q = 0; q < N; ++q) set(w, q, v[q]);
+    const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = (k * threads + tid) * V;
+      if (i < width) w[k].store(row + i, V, false);
+    }
+  }
+};
 
 // Sums of (p, q) over the block; `slot` alternates between calls, so that one
 // barrier is enough.
@@ -72,42 +126,26 @@ __device__ __forceinline__ float2 block_sum(float p, float q, float2 (*buf)[32],
 // One part of a row as it lies in memory.
 template <class T, class R, int V, int NV, int FORM>
 struct NormRow {
-  Pack<T, V> x[NV], gate[FORM == kResidual ? 1 : NV];
-  Pack<R, V> res[FORM == kGated ? 1 : NV];
+  Pack<T, V> x[NV], gate[NV];
+  Pack<R, V> res[NV];
 };
 
 template <class T, class R, int V, int NV, int FORM, int MAXT>
 __global__ void __launch_bounds__(MAXT) seq_norm_fwd_kernel(pt_norm_args a, int width, long long stride) {
+  using W = Words<V, NV>;
   __shared__ float2 buf[2][32];
-  const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
   const int c0 = static_cast<int>(blockIdx.x % a.groups) * width;
   const bool gated = FORM == kGated || (FORM == kAny && a.gate);
   const bool resid = FORM == kResidual || (FORM == kAny && a.residual);
   const bool scaled = FORM != kGated && a.scale;
-  float w[NV][V], sc[NV][V];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = (k * threads + tid) * V;
-    if (i < width) {
-      load_param<T, V>(a.weight, c0 + i, V, a.param_f32, w[k]);
-      if (scaled) load_param<T, V>(a.scale, c0 + i, V, a.param_f32, sc[k]);
-    }
-  }
+  F2 w[W::N], sc[W::N];
+  W::template params<T>(a.weight, c0, width, a.param_f32, w);
+  if (scaled) W::template params<T>(a.scale, c0, width, a.param_f32, sc);
   NormRow<T, R, V, NV, FORM> next;
   auto load = [&](long long row) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = (k * threads + tid) * V;
-      if (i < width) {
-        next.x[k].load(static_cast<const T*>(a.x) + row * a.x_row + c0 + i, V, true);
-        if constexpr (FORM != kResidual) {
-          if (gated) next.gate[k].load(static_cast<const T*>(a.gate) + row * a.gate_row + c0 + i, V, true);
-        }
-        if constexpr (FORM != kGated) {
-          if (resid) next.res[k].load(static_cast<const R*>(a.residual) + row * a.residual_row + c0 + i, V, true);
-        }
-      }
-    }
+    W::load(next.x, static_cast<const T*>(a.x) + row * a.x_row + c0, width);
+    if (gated) W::load(next.gate, static_cast<const T*>(a.gate) + row * a.gate_row + c0, width);
+    if (resid) W::load(next.res, static_cast<const R*>(a.residual) + row * a.residual_row + c0, width);
   };
   int slot = 0;
   long long row = blockIdx.x / a.groups;
@@ -116,96 +154,60 @@ __global__ void __launch_bounds__(MAXT) seq_norm_fwd_kernel(pt_norm_args a, int 
     NormRow<T, R, V, NV, FORM> in = next;
     if (row + stride < a.rows) load(row + stride);  // on its way while this row is worked on
     const long long o = row * a.dim + c0;
-    float r[NV][V], ss = 0.f;
+    F2 r[W::N], ss = 0;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = (k * threads + tid) * V;
-      if (i < width) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float u = in.x[k].f(v);
-          if constexpr (FORM != kResidual) {
-            if (gated) u *= siluf(in.gate[k].f(v));
-          }
-          if (scaled) u *= sc[k][v];
-          if constexpr (FORM != kGated) {
-            if (resid) {
-              // The stream that goes on is what is normalised: rounded to its type first.
-              in.res[k].set(v, in.res[k].f(v) + u);
-              u = in.res[k].f(v);
-            }
-          }
-          r[k][v] = u;
-          ss = fmaf(u, u, ss);
-        }
-        if constexpr (FORM != kGated) {
-          if (resid) in.res[k].store(static_cast<R*>(a.r) + o + i, V, true);
-        }
+    for (int q = 0; q < W::N; ++q) {
+      F2 u = W::get(in.x, q);
+      if (gated) {
+        const F2 g = W::get(in.gate, q);
+        u = mul2(u, mul2(g, sigmoid2(g)));
       }
-    }
-    const float rstd = rsqrtf(block_sum(ss, 0.f, buf, slot).x / static_cast<float>(width) + a.eps);
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = (k * threads + tid) * V;
-      if (i < width) {
-        Pack<T, V> out;
-#pragma unroll
-        for (int v = 0; v < V; ++v) out.set(v, r[k][v] * rstd * w[k][v]);
-        out.store(static_cast<T*>(a.y) + o + i, V, true);
+      if (scaled) u = mul2(u, sc[q]);
+      if (resid) {
+        // The stream that goes on is what is normalised: rounded to its type first.
+        W::set(in.res, q, add2(W::get(in.res, q), u));
+        u = W::get(in.res, q);
       }
+      r[q] = u;
+      ss = fma2(u, u, ss);
     }
+    if (resid) W::store(in.res, static_cast<R*>(a.r) + o, width);
+    const float rstd = rsqrtf(block_sum(sum2(ss), 0.f, buf, slot).x / static_cast<float>(width) + a.eps);
+    Pack<T, V> out[NV];
+#pragma unroll
+    for (int q = 0; q < W::N; ++q) W::set(out, q, mul2(mul2(r[q], same2(rstd)), w[q]));
+    W::store(out, static_cast<T*>(a.y) + o, width);
   }
 }
 
 template <class T, class R, int V, int NV, int FORM>
 struct NormGradRow {
-  Pack<T, V> dy[NV], x[NV], gate[FORM == kResidual ? 1 : NV];
-  Pack<R, V> r[FORM == kGated ? 1 : NV], dr[FORM == kGated ? 1 : NV];
+  Pack<T, V> dy[NV], x[NV], gate[NV];
+  Pack<R, V> r[NV], dr[NV];
 };
 
 template <class T, class R, int V, int NV, int FORM, int MAXT>
 __global__ void __launch_bounds__(MAXT) seq_norm_bwd_kernel(pt_norm_args a, float* part, int width, long long stride) {
+  using W = Words<V, NV>;
   __shared__ float2 buf[2][32];
-  const int tid = static_cast<int>(threadIdx.x), threads = static_cast<int>(blockDim.x);
   const int c0 = static_cast<int>(blockIdx.x % a.groups) * width;
   const bool gated = FORM == kGated || (FORM == kAny && a.gate);
   const bool resid = FORM == kResidual || (FORM == kAny && a.residual);
   const bool scaled = FORM != kGated && a.scale;
   const bool need_x = !resid || gated || (scaled && a.dscale);
   const bool more = FORM != kGated && a.dr;
-  float w[NV][V], sc[FORM == kGated ? 1 : NV][V], dw[NV][V], ds[FORM == kGated ? 1 : NV][V];
+  F2 w[W::N], sc[W::N], dw[W::N], ds[W::N];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = (k * threads + tid) * V;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      dw[k][v] = 0.f;
-      if constexpr (FORM != kGated) ds[k][v] = 0.f;
-    }
-    if (i < width) {
-      load_param<T, V>(a.weight, c0 + i, V, a.param_f32, w[k]);
-      if constexpr (FORM != kGated) {
-        if (scaled) load_param<T, V>(a.scale, c0 + i, V, a.param_f32, sc[k]);
-      }
-    }
-  }
+  for (int q = 0; q < W::N; ++q) dw[q] = ds[q] = 0;
+  W::template params<T>(a.weight, c0, width, a.param_f32, w);
+  if (scaled) W::template params<T>(a.scale, c0, width, a.param_f32, sc);
   NormGradRow<T, R, V, NV, FORM> next;
   auto load = [&](long long row) {
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = (k * threads + tid) * V;
-      if (i < width) {
-        next.dy[k].load(static_cast<const T*>(a.dy) + row * a.dy_row + c0 + i, V, true);
-        if (need_x) next.x[k].load(static_cast<const T*>(a.x) + row * a.x_row + c0 + i, V, true);
-        if constexpr (FORM != kResidual) {
-          if (gated) next.gate[k].load(static_cast<const T*>(a.gate) + row * a.gate_row + c0 + i, V, true);
-        }
-        if constexpr (FORM != kGated) {
-          if (resid) next.r[k].load(static_cast<const R*>(a.r) + row * a.dim + c0 + i, V, true);
-          if (more) next.dr[k].load(static_cast<const R*>(a.dr) + row * a.dr_row + c0 + i, V, true);
-        }
-      }
-    }
+    W::load(next.dy, static_cast<const T*>(a.dy) + row * a.dy_row + c0, width);
+    if (need_x) W::load(next.x, static_cast<const T*>(a.x) + row * a.x_row + c0, width);
+    if (gated) W::load(next.gate, static_cast<const T*>(a.gate) + row * a.gate_row + c0, width);
+    if (resid) W::load(next.r, static_cast<const R*>(a.r) + row * a.dim + c0, width);
+    if (more) W::load(next.dr, static_cast<const R*>(a.dr) + row * a.dr_row + c0, width);
   };
   int slot = 0;
   long long row = blockIdx.x / a.groups;
@@ -214,84 +216,52 @@ __global__ void __launch_bounds__(MAXT) seq_norm_bwd_kernel(pt_norm_args a, floa
     const NormGradRow<T, R, V, NV, FORM> in = next;
     if (row + stride < a.rows) load(row + stride);  // on its way while this row is worked on
     const long long o = row * a.dim + c0;
-    float r[NV][V], ss = 0.f, sv = 0.f;
+    F2 r[W::N], ss = 0, sv = 0;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = (k * threads + tid) * V;
-      if (i < width) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          float u;
-          if (resid) {
-            u = in.r[FORM == kGated ? 0 : k].f(v);
-          } else {
-            u = in.x[k].f(v);
-            if (gated) u *= siluf(in.gate[FORM == kResidual ? 0 : k].f(v));
-            if (scaled) u *= sc[FORM == kGated ? 0 : k][v];
-          }
-          r[k][v] = u;
-          ss = fmaf(u, u, ss);
-          sv = fmaf(in.dy[k].f(v) * w[k][v], u, sv);
+    for (int q = 0; q < W::N; ++q) {
+      F2 u;
+      if (resid) {
+        u = W::get(in.r, q);
+      } else {
+        u = W::get(in.x, q);
+        if (gated) {
+          const F2 g = W::get(in.gate, q);
+          u = mul2(u, mul2(g, sigmoid2(g)));
         }
+        if (scaled) u = mul2(u, sc[q]);
       }
+      r[q] = u;
+      ss = fma2(u, u, ss);
+      sv = fma2(mul2(W::get(in.dy, q), w[q]), u, sv);
     }
-    const float2 sums = block_sum(ss, sv, buf, slot);
+    const float2 sums = block_sum(sum2(ss), sum2(sv), buf, slot);
     const float inv = 1.f / static_cast<float>(width);
     const float rstd = rsqrtf(fmaf(sums.x, inv, a.eps)), mean = sums.y * inv * rstd;  // mean(v hat)
+    Pack<T, V> ox[NV], og[NV];
+    Pack<R, V> ores[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int i = (k * threads + tid) * V;
-      if (i < width) {
-        Pack<T, V> ox, og;
-        Pack<R, V> ores;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float hat = r[k][v] * rstd, y = in.dy[k].f(v);
-          dw[k][v] = fmaf(y, hat, dw[k][v]);
-          float d = rstd * (y * w[k][v] - hat * mean);
-          if constexpr (FORM != kGated) {
-            if (more) d += in.dr[k].f(v);
-            if (resid) ores.set(v, d);
-          }
-          float sig = 0.f, gv = 0.f, open = 1.f;
-          if constexpr (FORM != kResidual) {
-            if (gated) gv = in.gate[k].f(v), sig = sigmoidf(gv), open = gv * sig;
-          }
-          if constexpr (FORM != kGated) {
-            if (scaled) {
-              if (need_x) ds[k][v] = fmaf(d, in.x[k].f(v) * open, ds[k][v]);
-              d *= sc[k][v];
-            }
-          }
-          ox.set(v, d * open);
-          if constexpr (FORM != kResidual) {
-            if (gated) og.set(v, d * in.x[k].f(v) * silu_grad(gv, sig));
-          }
-        }
-        if (a.dx) ox.store(static_cast<T*>(a.dx) + o + i, V, true);
-        if constexpr (FORM != kResidual) {
-          if (a.dgate) og.store(static_cast<T*>(a.dgate) + o + i, V, true);
-        }
-        if constexpr (FORM != kGated) {
-          if (a.dresidual) ores.store(static_cast<R*>(a.dresidual) + o + i, V, true);
-        }
+    for (int q = 0; q < W::N; ++q) {
+      const F2 hat = mul2(r[q], same2(rstd)), y = W::get(in.dy, q);
+      dw[q] = fma2(y, hat, dw[q]);
+      F2 d = mul2(same2(rstd), fma2(hat, same2(-mean), mul2(y, w[q])));
+      if (more) d = add2(d, W::get(in.dr, q));
+      if (resid) W::set(ores, q, d);
+      F2 sig = 0, gv = 0, open = same2(1.f);
+      if (gated) gv = W::get(in.gate, q), sig = sigmoid2(gv), open = mul2(gv, sig);
+      if (scaled) {
+        if (need_x) ds[q] = fma2(d, mul2(W::get(in.x, q), open), ds[q]);
+        d = mul2(d, sc[q]);
       }
+      W::set(ox, q, mul2(d, open));
+      if (gated) W::set(og, q, mul2(mul2(d, W::get(in.x, q)), silu_grad2(gv, sig)));
     }
+    if (a.dx) W::store(ox, static_cast<T*>(a.dx) + o, width);
+    if (gated && a.dgate) W::store(og, static_cast<T*>(a.dgate) + o, width);
+    if (resid && a.dresidual) W::store(ores, static_cast<R*>(a.dresidual) + o, width);
   }
-  float* mine = part + static_cast<long long>(blockIdx.x / a.groups) * 2 * a.dim;
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int i = (k * threads + tid) * V;
-    if (i < width) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        mine[c0 + i + v] = dw[k][v];
-        if constexpr (FORM != kGated) {
-          if (a.dscale) mine[a.dim + c0 + i + v] = ds[k][v];
-        }
-      }
-    }
-  }
+  float* mine = part + static_cast<long long>(blockIdx.x / a.groups) * 2 * a.dim + c0;
+  W::put(dw, mine, width);
+  if (a.dscale) W::put(ds, mine + a.dim, width);
 }
 
 // Words per thread and the most threads of a block, which fix the registers
