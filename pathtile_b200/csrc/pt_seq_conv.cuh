@@ -444,7 +444,8 @@ inline int conv_width(const pt_conv_args& a, size_t e, int most) {
   for (int v = most; v > 1; v = v > 2 ? 2 : 1) {
     if (a.dim % v == 0 && conv_wide(a.x, a.x_batch, a.x_step, v, e) && conv_wide(a.dy, a.dy_batch, a.dy_step, v, e) &&
         conv_wide(a.state_in, 0, 0, v, e) && conv_wide(a.state_out, a.state_row, 0, v, e) && conv_wide(a.y, 0, 0, v, e) &&
-        conv_wide(a.dx, 0, 0, v, e) && conv_wide(a.dstate_in, 0, 0, v, e))
+        conv_wide(a.dx, 0, 0, v, e) && conv_wide(a.dstate_in, 0, 0, v, e) &&
+        conv_wide(a.dstate_out, 0, 0, v, e))
       return v;
   }
   return 1;
