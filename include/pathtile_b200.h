@@ -349,8 +349,9 @@ PT_API int pt_version(void);
  * (int32 [batch], NULL: all `len`) are the rows' valid steps, clamped to
  * 0..len: steps behind them are not read, their outputs (and gradients) are 0
  * and the state passes them unchanged.  No pointer needs more alignment than
- * its element type; 16-byte aligned rows move in wide words.  There is no
- * counterpart in the reference.
+ * its element type; 16-byte aligned rows move in wide words.  Outputs overlap
+ * neither inputs nor each other, but for a step's cache, which is both.  There
+ * is no counterpart in the reference.
  */
 #define PT_F32 0
 #define PT_BF16 1

@@ -83,6 +83,11 @@ int64_t cache_row(const Tensor& t, int64_t a, int64_t b, at::ScalarType type, co
   return row;
 }
 
+// The kernel wrote to it behind torch's back: what autograd saved of it is no longer that.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor slots_of(const Tensor& slots, int64_t batch, int64_t n, const Tensor& x) {
   if (!slots.defined()) {
     TORCH_CHECK_VALUE(n == batch, "state has ", n, " rows for a batch of ", batch, ": pass slots to choose among them");
@@ -92,8 +97,9 @@ Tensor slots_of(const Tensor& slots, int64_t batch, int64_t n, const Tensor& x) 
   return slots.contiguous();
 }
 
+// The kernels count a little past a row's end in 32 bits.
 int as_int(int64_t v, const char* what) {
-  TORCH_CHECK_VALUE(v <= INT_MAX, what, " is too large: ", v);
+  TORCH_CHECK_VALUE(v <= INT_MAX - 4096, what, " is too large: ", v);
   return static_cast<int>(v);
 }
 
@@ -236,7 +242,7 @@ variable_list causal_conv(const Tensor& x, const Tensor& w, const OptTensor& bia
 Tensor causal_conv_step(const Tensor& state, const Tensor& x_, const Tensor& w_, const OptTensor& bias_, bool silu,
                         const OptTensor& slots_) {
   const Tensor bias = dense(given(bias_));
-  refuse_grad("causal_conv_step", {x_, w_, bias});
+  refuse_grad("causal_conv_step", {state, x_, w_, bias});
   conv_check(x_, w_, bias, 2);
   const int64_t row = cache_row(state, w_.size(1) - 1, x_.size(1), x_.scalar_type(), x_);
   const Tensor slots = slots_of(given(slots_), x_.size(0), state.size(0), x_);
@@ -247,6 +253,7 @@ Tensor causal_conv_step(const Tensor& state, const Tensor& x_, const Tensor& w_,
   a.cache_rows = as_int(state.size(0), "state");
   a.state_out = out_ptr(state), a.state_row = row, a.slots = as<int>(slots), a.y = out_ptr(y);
   check(pt_causal_conv_step(&a, call.stream), "pt_causal_conv_step");
+  written(state);
   return y;
 }
 
@@ -386,7 +393,7 @@ Tensor selective_scan_step(const Tensor& state, const Tensor& x, const Tensor& d
                            const Tensor& C, const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias,
                            bool softplus, const OptTensor& slots_) {
   ScanIn v{x, dt, A, B, C, given(D), given(z), given(dt_bias), Tensor(), Tensor()};
-  refuse_grad("selective_scan_step", {v.x, v.dt, v.A, v.B, v.C, v.D, v.z, v.dt_bias});
+  refuse_grad("selective_scan_step", {state, v.x, v.dt, v.A, v.B, v.C, v.D, v.z, v.dt_bias});
   scan_check(v, 2);
   const int64_t row = cache_row(state, A.size(0), A.size(1), at::kFloat, x);
   const Tensor slots = slots_of(given(slots_), x.size(0), state.size(0), x);
@@ -397,6 +404,7 @@ Tensor selective_scan_step(const Tensor& state, const Tensor& x, const Tensor& d
   a.cache_rows = as_int(state.size(0), "state");
   a.hlast = out_as<float>(state), a.h_row = row, a.slots = as<int>(slots), a.y = out_ptr(y);
   check(pt_scan_step(&a, call.stream), "pt_scan_step");
+  written(state);
   return y;
 }
 

@@ -84,7 +84,9 @@ class SelectiveBlock(nn.Module):
         """Branch output and residual stream for ``x[batch, length, hidden]``.
 
         ``cache`` (one row per batch row) holds what came before and is brought
-        up to each row's end; ``lengths`` as in :func:`selective_scan`.
+        up to each row's end: in place, or, while gradients are recorded, with
+        new tensors (no gradient passes through it); ``lengths`` as in
+        :func:`selective_scan`.
         """
         h, residual = self._enter(x, residual)
         u, z = self.in_proj(h).chunk(2, dim=-1)
@@ -98,7 +100,9 @@ class SelectiveBlock(nn.Module):
                            initial_state=cache.state if keep else None, return_final_state=keep, lengths=lengths)
         if keep:
             y, state = y
-            with torch.no_grad():
+            if torch.is_grad_enabled():  # what the backward pass has saved must stay: the cache gets new tensors
+                cache.window, cache.state = window.detach(), state.detach()
+            else:
                 cache.window.copy_(window)
                 cache.state.copy_(state)
         return self._leave(y, z), residual

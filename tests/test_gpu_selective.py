@@ -96,6 +96,21 @@ def test_prompts_then_tokens_through_a_cache(cuda_device):
         assert not big.state[[1, 2, 4, 5, 6]].any() and not big.window[[1, 2, 4, 5, 6]].any()
 
 
+def test_training_in_pieces_through_a_cache(cuda_device):
+    """The second piece starts from the first one's end; its gradients stay within it."""
+    torch.manual_seed(8)
+    block = SelectiveBlock(16, 8).to(cuda_device)
+    x = torch.randn(2, 12, 16, device=cuda_device)
+    cache = block.make_cache(2)
+    first, _ = block(x[:, :5], cache=cache)
+    second, _ = block(x[:, 5:], cache=cache)
+    (first.square().sum() + second.square().sum()).backward()
+    assert all(torch.isfinite(p.grad).all() for p in block.parameters() if p.grad is not None)
+    with torch.no_grad():
+        whole, _ = block(x)
+    near(torch.cat((first, second), 1), whole.double(), "two pieces")
+
+
 def test_a_padded_batch_of_prompts(cuda_device):
     torch.manual_seed(5)
     block = SelectiveBlock(32, 16).to(cuda_device)

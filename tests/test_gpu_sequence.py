@@ -339,6 +339,19 @@ def test_slots_past_the_cache_and_named_twice_are_refused(cuda_device, slots, bi
     assert ops.device_error(clear=True) == bit
 
 
+def test_a_step_counts_as_a_change_of_its_cache(cuda_device):
+    """Autograd sees that a saved cache was changed, and a cache that asks for a gradient is refused."""
+    m = Maker(cuda_device, 34)
+    state, x, w = m(2, 3, 8), m(2, 8), m(8, 4)
+    leaf = m(2, 3, 8).requires_grad_()
+    product = (leaf * state).sum()  # saves state
+    pt.causal_conv_step(state, x, w)
+    with pytest.raises(RuntimeError, match="inplace"):
+        product.backward()
+    with pytest.raises(ValueError, match="no_grad"):
+        pt.causal_conv_step(state.requires_grad_(), x, w)
+
+
 def test_offsets_past_32_bits(cuda_device):
     """A cache whose last rows lie more than 2^32 bytes and 2^31 elements in, and one layer's rows of it."""
     d, n, rows = 1024, 64, 33000
@@ -422,6 +435,68 @@ def test_fused_norm_on_strided_rows(cuda_device):
     one = ref.norm(leaf, w, dy=torch.ones(1, 65, device=cuda_device))
     size = ref.norm(leaf, w, dy=torch.ones(1, 65, device=cuda_device), absolute=True)
     close(grad, 8 * one["dx"], 8 * size["dx"], 100, "dx")
+
+
+# ---------------------------------------------------------------- alignment
+def shifted(t):
+    """The same values, contiguous, from the second element of a buffer on."""
+    if t is None or t.dtype == torch.int32:
+        return t
+    buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    out = buf[1:].view(t.shape)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_tensors_that_begin_at_an_odd_element(cuda_device, dtype):
+    m = Maker(cuda_device, 45)
+    b, l, d, n = 3, 21, 64, 16
+    x, w, bias, state = m(b, l, d, dtype=dtype), m(d, 4), m(d), m(b, 3, d, dtype=dtype)
+    dy, dlast = m(b, l, d, dtype=dtype), m(b, 3, d, dtype=dtype)
+
+    def conv(args, grads):
+        leaves = [t.detach().requires_grad_() for t in args]
+        y, last = pt.causal_conv(*leaves[:3], silu=True, initial_state=leaves[3], return_final_state=True)
+        return [y.detach(), last.detach(), *torch.autograd.grad([y, last], leaves, grads)]
+
+    plain = conv((x, w, bias, state), (dy, dlast))
+    every = (x, w, bias, state, dy, dlast)
+    for i in range(len(every)):  # one at a time: one alone decides the width for all
+        args = [shifted(t) if j == i else t for j, t in enumerate(every)]
+        for p, q in zip(conv(args[:4], args[4:]), plain):
+            torch.testing.assert_close(p, q, rtol=1e-5 if dtype == F32 else 1e-2, atol=1e-5 if dtype == F32 else 1e-2)
+    one, two = state.clone(), shifted(state)
+    assert torch.equal(pt.causal_conv_step(one, x[:, 0], w, bias), pt.causal_conv_step(two, shifted(x[:, 0]), shifted(w), shifted(bias)))
+    assert torch.equal(one, two)
+
+    v = scan_inputs(m, b, l, d, n, 1, dtype, True, True, True, True, False)
+    gy, gl = m(b, l, d, dtype=dtype), m(b, d, n)
+
+    def scan(v, grads):
+        v = {k: t.detach().requires_grad_() for k, t in v.items()}
+        y, last = pt.selective_scan(**v, dt_softplus=True, return_final_state=True)
+        return [y.detach(), last.detach(), *torch.autograd.grad([y, last], list(v.values()), grads)]
+
+    for p, q in zip(scan({k: shifted(t) for k, t in v.items()}, (shifted(gy), shifted(gl))), scan(v, (gy, gl))):
+        assert torch.equal(p, q)
+    now = {k: v[k][:, 0].contiguous() for k in ("x", "dt", "B", "C", "z")} | {k: v[k] for k in ("A", "D", "dt_bias")}
+    one, two = v["initial_state"].clone(), shifted(v["initial_state"])
+    assert torch.equal(pt.selective_scan_step(one, **now, dt_softplus=True),
+                       pt.selective_scan_step(two, **{k: shifted(t) for k, t in now.items()}, dt_softplus=True))
+    assert torch.equal(one, two)
+
+    parts = dict(x=m(9, d, dtype=dtype), weight=m(d), gate=m(9, d, dtype=dtype), residual=m(9, d), scale=m(d))
+    gy, gr = m(9, d, dtype=dtype), m(9, d)
+
+    def norm(v, grads):
+        v = {k: t.detach().requires_grad_() for k, t in v.items()}
+        outs = pt.fused_norm(**v)
+        return [*(t.detach() for t in outs), *torch.autograd.grad(outs, list(v.values()), grads)]
+
+    plain = norm(parts, (gy, gr))
+    for p, q in zip(norm({k: shifted(t) for k, t in parts.items()}, (shifted(gy), shifted(gr))), plain):
+        torch.testing.assert_close(p, q, rtol=1e-5 if p.dtype == F32 else 1e-2, atol=1e-4 if p.dtype == F32 else 1e-2)
 
 
 # ---------------------------------------------------------------- infinities and NaN
