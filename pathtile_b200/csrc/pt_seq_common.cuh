@@ -168,8 +168,6 @@ __device__ __forceinline__ float rcp(float x) {
 // 1 / (1 + e^-v): the reciprocal of infinity is 0, so large negative v need no care.
 __device__ __forceinline__ float sigmoidf(float v) { return rcp(1.f + ex2(v * -kLog2e)); }
 __device__ __forceinline__ float siluf(float v) { return v * sigmoidf(v); }
-// d silu(v) / dv, with s = sigmoid(v).
-__device__ __forceinline__ float silu_grad(float v, float s) { return s * fmaf(v, 1.f - s, 1.f); }
 
 __device__ __forceinline__ F2 ex2x2(F2 x) { return pack2(ex2(lo2(x)), ex2(hi2(x))); }
 __device__ __forceinline__ F2 same2(float v) { return pack2(v, v); }

@@ -28,8 +28,9 @@ constexpr int kConvThreads = 128;
 
 // Blocks per SM that the registers are kept down for, and steps whose loads are
 // under way together.  One wave of long stretches beats several waves of short
-// ones (8 x 2048 x 4096 bf16, 4 taps: forward 60 against 69 us with four waves;
-// backward 129 us, 200 us at the 146 registers that it would take by itself).
+// ones (8 x 2048 x 4096 bf16, 4 taps, before the loops were split: forward 60
+// against 69 us with four waves; backward 129 us, 200 us at the 146 registers that
+// it would take by itself).  Now 52 us (5.2 TB/s) and 100 us (4.0 TB/s).
 // Narrow words (rows that are not aligned) need more threads and steps for the
 // same bytes on their way.
 template <int V>

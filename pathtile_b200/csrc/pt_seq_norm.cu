@@ -12,6 +12,10 @@
 //   dr = rstd (v - hat mean(v hat)) + dr_in;  dx = dr scale silu(gate), ...
 // mean(r^2) and mean(v r) come from one reduction.  dweight and dscale: one
 // partial sum per block, added in a fixed order by a second kernel.
+//
+// 16384 x 4096 in 8 groups, gated, bf16: forward 65 us (6.2 TB/s), backward 130
+// (5.2 TB/s), with issue slots 70 % busy.  8191 x 1027, residual in fp32 and scale,
+// single elements: 24 and 53 us.
 #include <type_traits>
 
 #include "pt_seq.h"

@@ -368,6 +368,48 @@ def test_offsets_past_32_bits(cuda_device):
     assert torch.equal(y, want) and torch.equal(cache[rows - 1], small[0]) and torch.equal(cache[0], small[1])
 
 
+def test_tensors_of_more_than_two_billion_elements(cuda_device):
+    """The far end of operands past 2^31 elements, forward and backward: what a short call on the last steps gives
+    (the scan forgets the earlier ones: 100 steps of decay e^-2 leave e^-200)."""
+    l, d, n, end = 530_000, 4096, 4, 200
+    m = Maker(cuda_device, 35)
+
+    def big(*shape):
+        return torch.randn(*shape, generator=m.gen, device=cuda_device, dtype=BF16)
+
+    x, w, bias = big(1, l, d), m(d, 4), m(d)
+    assert x.numel() > 2 ** 31
+    leaf = x.requires_grad_()
+    y = pt.causal_conv(leaf, w, bias, silu=True)
+    dy = big(1, l, d)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    tail = x[:, -end:].detach().clone().requires_grad_()
+    want = pt.causal_conv(tail, w, bias, silu=True)
+    dtail, = torch.autograd.grad(want, tail, dy[:, -end:])
+    assert torch.equal(y[:, -end + 3:], want[:, 3:]) and torch.equal(dx[:, -end + 3:], dtail[:, 3:])
+    del y, dx
+    torch.cuda.empty_cache()
+
+    rows = x.detach().view(l, d)
+    gain = m(d).requires_grad_()
+    y = pt.fused_norm(rows, gain, gate=dy.view(l, d))
+    assert torch.equal(y[-9:], pt.fused_norm(rows[-9:].clone(), gain, gate=dy.view(l, d)[-9:].clone()))
+    del y
+    torch.cuda.empty_cache()
+
+    A = torch.full((d, n), -2.0, device=cuda_device)
+    B, C = m(1, l, n, dtype=BF16), m(1, l, n, dtype=BF16)
+    dt = torch.ones((), dtype=BF16, device=cuda_device).expand(1, l, d)
+    y, last = pt.selective_scan(leaf, dt, A, B, C, return_final_state=True)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    part = [t[:, -end:] for t in (dt, B, C)]
+    want, state = pt.selective_scan(tail, part[0], A, part[1], part[2], return_final_state=True)
+    dtail, = torch.autograd.grad(want, tail, dy[:, -end:])
+    # Both sides are rounded once to bf16: 2^-8 of the value each.
+    for got, w in ((y[:, -100:], want[:, -100:]), (last, state), (dx[:, -100:], dtail[:, -100:])):
+        torch.testing.assert_close(got, w, rtol=2.0 ** -7, atol=2.0 ** -7)
+
+
 # ---------------------------------------------------------------- norm
 NORM = [
     # shape, groups, dtype, residual's dtype, gate, scale, parameters' dtype
