@@ -1,5 +1,6 @@
 // pt_seq_api.cu -- C entry points of the sequence operators: argument checks,
 // the scan's plan and dispatch by type.
+#include <climits>
 #include <type_traits>
 
 #include "pt_seq.h"
@@ -29,12 +30,14 @@ namespace {
 constexpr int kTileSteps = 16;  // kTile of pt_seq_scan.cuh
 
 int status(cudaError_t e) { return e == cudaSuccess ? PT_OK : seq_cuda_fail(e); }
+// The kernels count a little past a row's end in 32 bits.
+bool length_ok(int len) { return len <= INT_MAX - 4096; }
 bool type_ok(int t) { return t == PT_F32 || t == PT_BF16 || t == PT_F16; }
 
 int check(const pt_conv_args* a) {
   if (!a || !type_ok(a->dtype)) return PT_ERR_ARGS;
   if (a->batch < 0 || a->len < 0 || a->dim < 1 || a->taps < 1) return PT_ERR_ARGS;
-  if (a->taps > PT_CONV_MAX_TAPS) return PT_ERR_UNSUPPORTED;
+  if (a->taps > PT_CONV_MAX_TAPS || !length_ok(a->len)) return PT_ERR_UNSUPPORTED;
   if (a->batch > 0 && (!a->w || (a->len > 0 && !a->x))) return PT_ERR_ARGS;
   return PT_OK;
 }
@@ -42,7 +45,7 @@ int check(const pt_conv_args* a) {
 int check(const pt_scan_args* a) {
   if (!a || !type_ok(a->dtype)) return PT_ERR_ARGS;
   if (a->batch < 0 || a->len < 0 || a->dim < 1 || a->state < 1 || a->groups < 1 || a->dim % a->groups) return PT_ERR_ARGS;
-  if (a->state > PT_SCAN_MAX_STATE) return PT_ERR_UNSUPPORTED;
+  if (a->state > PT_SCAN_MAX_STATE || !length_ok(a->len)) return PT_ERR_UNSUPPORTED;
   if (a->batch > 0 && (!a->A || (a->len > 0 && (!a->x || !a->dt || !a->B || !a->C)))) return PT_ERR_ARGS;
   return PT_OK;
 }

@@ -58,6 +58,14 @@ def test_conv_argument_checks(native_lib, kw, status):
     assert native_lib.pt_causal_conv_bwd_workspace_bytes(conv_args(**kw)) == 0
 
 
+def test_lengths_that_leave_no_room_to_count_past_a_rows_end(native_lib):
+    for n in (2 ** 31 - 1, 2 ** 31 - 4096):
+        assert native_lib.pt_causal_conv(conv_args(len=n), NULL) == _lib.PT_ERR_UNSUPPORTED
+        assert native_lib.pt_causal_conv_bwd(conv_args(len=n), NULL, 0, NULL) == _lib.PT_ERR_UNSUPPORTED
+        assert native_lib.pt_scan(scan_args(len=n), NULL, 0, NULL) == _lib.PT_ERR_UNSUPPORTED
+        assert native_lib.pt_scan_bwd(scan_args(len=n), NULL, 0, NULL) == _lib.PT_ERR_UNSUPPORTED
+
+
 def test_step_argument_checks(native_lib):
     assert native_lib.pt_causal_conv(NULL, NULL) == _lib.PT_ERR_ARGS
     assert native_lib.pt_causal_conv(conv_args(y=NULL), NULL) == _lib.PT_ERR_ARGS
