@@ -70,13 +70,18 @@ class SelectiveBlock(nn.Module):
         dt, B, C = self.x_proj(u).split((self.dt_rank, self.states, self.states), dim=-1)
         return F.linear(dt, self.dt_proj.weight), B, C
 
+    def _scan_params(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """A, D and the bias of dt, which the scan takes in float32 whatever the module's type."""
+        return -torch.exp(self.log_A.float()), self.D.float(), self.dt_bias.float()
+
     def _leave(self, y: torch.Tensor, z: torch.Tensor) -> torch.Tensor:
         return self.out_proj(fused_norm(y, self.out_norm_weight, gate=z, groups=self.norm_groups, eps=self.eps))
 
-    def make_cache(self, rows: int) -> SelectiveCache:
-        """An empty cache of ``rows`` sequences, on the block's device."""
+    def make_cache(self, rows: int, dtype: torch.dtype | None = None) -> SelectiveCache:
+        """An empty cache of ``rows`` sequences, on the block's device.  ``dtype``: the
+        type the block computes in, its weights' own unless it runs under autocast."""
         w = self.in_proj.weight
-        return SelectiveCache(w.new_zeros(rows, self.taps - 1, self.inner),
+        return SelectiveCache(w.new_zeros(rows, self.taps - 1, self.inner, dtype=dtype),
                               torch.zeros(rows, self.inner, self.states, dtype=torch.float32, device=w.device))
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
@@ -96,7 +101,8 @@ class SelectiveBlock(nn.Module):
         if keep:
             u, window = u
         dt, B, C = self._operands(u)
-        y = selective_scan(u, dt, -torch.exp(self.log_A), B, C, self.D, None, self.dt_bias, dt_softplus=True,
+        A, D, dt_bias = self._scan_params()
+        y = selective_scan(u, dt, A, B, C, D, None, dt_bias, dt_softplus=True,
                            initial_state=cache.state if keep else None, return_final_state=keep, lengths=lengths)
         if keep:
             y, state = y
@@ -115,6 +121,6 @@ class SelectiveBlock(nn.Module):
         u, z = self.in_proj(h).chunk(2, dim=-1)
         u = causal_conv_step(cache.window, u, self.conv_weight, self.conv_bias, silu=True, slots=slots)
         dt, B, C = self._operands(u)
-        y = selective_scan_step(cache.state, u, dt, -torch.exp(self.log_A), B, C, self.D, None, self.dt_bias,
-                                dt_softplus=True, slots=slots)
+        A, D, dt_bias = self._scan_params()
+        y = selective_scan_step(cache.state, u, dt, A, B, C, D, None, dt_bias, dt_softplus=True, slots=slots)
         return self._leave(y, z), residual

@@ -128,6 +128,37 @@ def test_a_padded_batch_of_prompts(cuda_device):
             near(cache.window[i], one.window[0].double(), f"window {i}")
 
 
+def test_a_block_in_bfloat16_and_under_autocast(cuda_device):
+    """Two bfloat16 products of 32 and 64 terms, two more on what they made and six roundings between: 2^-8 each of
+    about the largest value, twelve of them 0.047."""
+    torch.manual_seed(7)
+    block = SelectiveBlock(32, 16).to(cuda_device)
+    x = torch.randn(2, 19, 32, device=cuda_device)
+    with torch.no_grad():
+        whole, _ = block(x)
+        runs = {}
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            cache = block.make_cache(2, dtype=torch.bfloat16)
+            y, _ = block(x[:, :18], cache=cache)
+            token, _ = block.step(x[:, 18], cache)
+            runs["autocast"] = torch.cat((y, token[:, None]), 1)
+    half = SelectiveBlock(32, 16).to(cuda_device)
+    half.load_state_dict(block.state_dict())
+    half.bfloat16()
+    y, _ = half(x.bfloat16())
+    y.float().square().sum().backward()
+    assert all(p.grad is not None and p.grad.dtype == torch.bfloat16 and p.grad.isfinite().all() for p in half.parameters())
+    with torch.no_grad():
+        cache = half.make_cache(2)
+        first, _ = half(x[:, :18].bfloat16(), cache=cache)
+        token, _ = half.step(x[:, 18].bfloat16(), cache)
+        runs["bfloat16"] = torch.cat((first, token[:, None]), 1)
+    runs["bfloat16, whole"] = y.detach()
+    for name, got in runs.items():
+        off = float((got.float() - whole).abs().max() / whole.abs().max())
+        assert got.dtype == torch.bfloat16 and off <= 12 * 2.0 ** -8, f"{name}: {off:.3g}"
+
+
 def test_the_model_trains_with_selective_blocks(cuda_device):
     torch.manual_seed(6)
     model = s4conv.Model(state_dim=16, hidden_dim=64, num_blocks=2, block="selective").to(cuda_device)
