@@ -563,9 +563,9 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
   meet<TEAM>();
   for (int k = 0; k < tiles; ++k) {
     const int st = k & 1;
-    if (a.checkpoints)
-      store_states(a.checkpoints + (b * ckpt_row + t0 / kTile + k) * a.dim * a.state, a, me, h);
-    {
+    if (t0 + k * kTile < len) {  // behind the row's end nothing moves
+      if (a.checkpoints)
+        store_states(a.checkpoints + (b * ckpt_row + t0 / kTile + k) * a.dim * a.state, a, me, h);
       // Decays of the next pair of steps are computed while this pair is scanned, and its sums cross the lanes one
       // pair later: no instruction waits for the one before it.
       F2 e[2][2][2];
@@ -802,16 +802,19 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
         if (part_bc) {
           // [block of the group's channels][batch][len][group][2 * states]
           constexpr int kRow = 2 * P::kStates, kEach = 4;
-          const int tile = t_out - me.tr, rows = min(kTile, t1 - tile);
+          const int tile = t_out - me.tr, rows = min(kTile, t1 - tile), valid = len - tile;
           const long long row = (static_cast<long long>(at.cb % dm.cblocks) * a.batch + b) * a.len + tile;
 #pragma unroll 1
           for (int i = (tid - kScanners) * kEach; i < rows * kRow; i += TEAM::kStagers * kEach) {
             const int q = i / kRow, k2 = i % kRow;
-            float4 s = *reinterpret_cast<const float4*>(&sm.red[st][0][q][k2]);
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (q < valid) {
+              s = *reinterpret_cast<const float4*>(&sm.red[st][0][q][k2]);
 #pragma unroll
-            for (int w = 1; w < kScanWarps; ++w) {
-              const float4 m = *reinterpret_cast<const float4*>(&sm.red[st][w][q][k2]);
-              s.x += m.x, s.y += m.y, s.z += m.z, s.w += m.w;
+              for (int w = 1; w < kScanWarps; ++w) {
+                const float4 m = *reinterpret_cast<const float4*>(&sm.red[st][w][q][k2]);
+                s.x += m.x, s.y += m.y, s.z += m.z, s.w += m.w;
+              }
             }
             *reinterpret_cast<float4*>(part_bc + ((row + q) * a.groups + at.g) * kRow + k2) = s;
           }
@@ -849,6 +852,7 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
   sm.accA[0][tid] = sm.accA[1][tid] = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool quads = (a.state & 3) == 0 && (reinterpret_cast<uintptr_t>(a.checkpoints) & 15) == 0;
   for (int b = chunk; b < a.batch; b += dm.row_chunks) {
+    const int len = scan_row_length(a, b);
     auto fetch = [&](int k) {
       const float* ck = a.checkpoints + (b * ckpt_row + tile_of(k) / kTile) * all;
       if (quads) {
@@ -883,6 +887,10 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
         first[c][0] = h[c][0] = v.x, first[c][1] = h[c][1] = v.y;
       }
       if (k + 1 < tiles) fetch(k + 1);
+      if (tile_of(k) >= len) {  // behind the row's end: no gradients, and no checkpoint was kept
+        meet<TEAM>();
+        continue;
+      }
       // The states at the later parts' starts.
 #pragma unroll 1
       for (int sub = 0; sub < kTile / kSub - 1; ++sub) {

@@ -573,6 +573,35 @@ def test_infinities_and_nans_stay_in_their_channel(cuda_device):
     assert got[1].isnan().all() and torch.equal(got[[0, 2, 3]], want[[0, 2, 3]])
 
 
+@pytest.mark.parametrize("l,n", [(20, 16), (50, 6), (300, 24)])
+def test_an_empty_rows_state_reaches_no_sum(cuda_device, l, n):
+    """What a row without valid steps carries from its initial to its final state, finite or not, is in no other
+    row's gradient and in none that sums over rows."""
+    m = Maker(cuda_device, 53)
+    v = scan_inputs(m, 3, l, 24, n, 1, F32, True, True, True, True, False)
+    w, window = m(24, 4), m(3, 3, 24)
+    dy, dlast, dwindow = m(3, l, 24), m(3, 24, n), m(3, 3, 24)
+    lengths = torch.tensor([l, 0, l // 3], dtype=torch.int32, device=cuda_device)
+
+    def grads(state, dlast, window, dwindow):
+        leaves = [t.detach().requires_grad_() for t in {**v, "initial_state": state}.values()]
+        y, last = pt.selective_scan(**dict(zip(v, leaves)), dt_softplus=True, lengths=lengths, return_final_state=True)
+        out = [y.detach(), last.detach(), *torch.autograd.grad([y, last], leaves, [dy, dlast])]
+        leaves = [t.detach().requires_grad_() for t in (v["x"], w, window)]
+        y, last = pt.causal_conv(*leaves[:2], initial_state=leaves[2], lengths=lengths, return_final_state=True)
+        return [*out, y.detach(), last.detach(), *torch.autograd.grad([y, last], leaves, [dy, dwindow])]
+
+    want = grads(v["initial_state"], dlast, window, dwindow)
+    odd = [t.clone() for t in (v["initial_state"], dlast, window, dwindow)]
+    for t in odd:
+        t[1, ::2], t[1, 1::2] = float("nan"), float("inf")
+    for i, (got, one) in enumerate(zip(grads(*odd), want, strict=True)):
+        if got.shape[0] == 3 and not torch.isfinite(got).all():  # a state, or its gradient: as it came
+            assert torch.equal(got[1].isnan(), odd[0 if got.shape == odd[0].shape else 2][1].isnan()), i
+            got, one = got[[0, 2]], one[[0, 2]]
+        assert torch.equal(got, one), i
+
+
 def test_far_decays_and_large_steps(cuda_device):
     """Steps that forget everything, steps of no duration, and rates of zero."""
     m = Maker(cuda_device, 52)
