@@ -403,6 +403,10 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
   meet<TEAM>();
   for (int k = 0; k < tiles; ++k) {
     const int st = k & 1;
+    if (tile_of(k) >= len) {  // behind the row's end nothing moves
+      meet<TEAM>();
+      continue;
+    }
 #pragma unroll 8
     for (int q = 0; q < kTile; ++q) {
       const int i = REV ? kTile - 1 - q : q;
