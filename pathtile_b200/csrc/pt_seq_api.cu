@@ -42,10 +42,15 @@ int check(const pt_conv_args* a) {
   return PT_OK;
 }
 
-int check(const pt_scan_args* a) {
+int check_sizes(const pt_scan_args* a) {
   if (!a || !type_ok(a->dtype)) return PT_ERR_ARGS;
   if (a->batch < 0 || a->len < 0 || a->dim < 1 || a->state < 1 || a->groups < 1 || a->dim % a->groups) return PT_ERR_ARGS;
-  if (a->state > PT_SCAN_MAX_STATE || !length_ok(a->len)) return PT_ERR_UNSUPPORTED;
+  return a->state > PT_SCAN_MAX_STATE || !length_ok(a->len) ? PT_ERR_UNSUPPORTED : PT_OK;
+}
+
+int check(const pt_scan_args* a) {
+  const int rc = check_sizes(a);
+  if (rc != PT_OK) return rc;
   if (a->batch > 0 && (!a->A || (a->len > 0 && (!a->x || !a->dt || !a->B || !a->C)))) return PT_ERR_ARGS;
   return PT_OK;
 }
@@ -163,7 +168,7 @@ int pt_causal_conv_step(const pt_conv_args* a, void* stream) {
 }
 
 size_t pt_scan_checkpoint_bytes(const pt_scan_args* a) {
-  if (check(a) != PT_OK) return 0;
+  if (check_sizes(a) != PT_OK) return 0;
   return sizeof(float) * static_cast<size_t>(a->batch) * cdiv(a->len, kTileSteps) * a->dim * a->state;
 }
 

@@ -19,8 +19,12 @@ of that device; calls allocate their outputs and scratch from the current
 stream's allocator, so they may be captured into CUDA graphs.  (As with every
 differentiable operation, a backward pass is captured only while no eager graph
 of the same leaves is alive: autograd would synchronise with that graph's
-stream, which ends the capture.)  There is no counterpart in the reference, and
-no fallback.
+stream, which ends the capture.)  Each call is an operator of torch's dispatcher
+(``torch.ops.pathtile_b200``, there from the first call on), backward passes too: ``torch.jit.trace``,
+``make_fx`` and dispatch modes record it as one, and on meta tensors it gives
+shapes only.  There are no derivatives in forward mode and no rules for
+``torch.func``'s transforms: a tensor with a tangent, and a transform, are refused.
+There is no counterpart in the reference, and no fallback.
 """
 from __future__ import annotations
 
