@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kConvThreads, kConvFwdBlocks<V>)
 #pragma unroll
       for (int i = 0; i < Packed<V>::N; ++i) {
         s.p[i] = taps.pre(win, i);
-        if (a.silu) s.p[i] = mul2(s.p[i], sigmoid2(s.p[i]));
+        if (a.silu) s.p[i] = mul2(s.p[i], sigmoid2<T>(s.p[i]));
       }
       Pack<T, V> out;
       s.to(out);
@@ -252,7 +252,7 @@ __device__ __forceinline__ void conv_bwd_stretch(const pt_conv_args& a, const Ta
 #pragma unroll
     for (int i = 0; i < Packed<V>::N; ++i) {
       if (a.silu) {
-        const F2 pre = taps.pre(win, i), sig = sigmoid2(pre);
+        const F2 pre = taps.pre(win, i), sig = sigmoid2<T>(pre);
         g.p[i] = mul2(g.p[i], silu_grad2(pre, sig));
       }
       // Steps behind the row's end have no output; their window may hold anything.
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kConvThreads) seq_conv_step_kernel(pt_conv_arg
     float s = bias.v[v];
 #pragma unroll
     for (int j = 0; j < K; ++j) s = fmaf(w.v[v * K + j], win[j].f(v), s);
-    out.set(v, a.silu ? s * lo2(sigmoid2(pack2(s, s))) : s);
+    out.set(v, a.silu ? s * lo2(sigmoid2<T>(pack2(s, s))) : s);
   }
   out.store(y, V, true);
 #pragma unroll

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(MAXT) seq_norm_fwd_kernel(pt_norm_args a, int 
       F2 u = W::get(in.x, q);
       if (gated) {
         const F2 g = W::get(in.gate, q);
-        u = mul2(u, mul2(g, sigmoid2(g)));
+        u = mul2(u, mul2(g, sigmoid2<T>(g)));
       }
       if (scaled) u = mul2(u, sc[q]);
       if (resid) {
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(MAXT) seq_norm_bwd_kernel(pt_norm_args a, floa
         u = W::get(in.x, q);
         if (gated) {
           const F2 g = W::get(in.gate, q);
-          u = mul2(u, mul2(g, sigmoid2(g)));
+          u = mul2(u, mul2(g, sigmoid2<T>(g)));
         }
         if (scaled) u = mul2(u, sc[q]);
       }
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(MAXT) seq_norm_bwd_kernel(pt_norm_args a, floa
       if (more) d = add2(d, W::get(in.dr, q));
       if (resid) W::set(ores, q, d);
       F2 sig = 0, gv = 0, open = same2(1.f);
-      if (gated) gv = W::get(in.gate, q), sig = sigmoid2(gv), open = mul2(gv, sig);
+      if (gated) gv = W::get(in.gate, q), sig = sigmoid2<T>(gv), open = mul2(gv, sig);
       if (scaled) {
         if (need_x) ds[q] = fma2(d, mul2(W::get(in.x, q), open), ds[q]);
         d = mul2(d, sc[q]);

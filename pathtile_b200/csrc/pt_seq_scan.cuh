@@ -366,12 +366,12 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
 #pragma unroll
         for (int i = 0; i < me.kPairs; ++i) {
           d[i] = add2(dt.pair(i), bias[i]);
-          if (a.dt_softplus) d[i] = softplus2(d[i]);
+          if (a.dt_softplus) d[i] = softplus2<T>(d[i]);
           v[i] = in.pair(i);
           if constexpr (REV) {
             if (gated) {
               const F2 zi = z.pair(i);
-              v[i] = mul2(v[i], mul2(zi, sigmoid2(zi)));
+              v[i] = mul2(v[i], mul2(zi, sigmoid2<T>(zi)));
             }
           } else {
             v[i] = mul2(v[i], d[i]);
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
 #pragma unroll
         for (int i = 0; i < me.kPairs; ++i) {
           d[i] = add2(dt.pair(i), bias[i]);
-          if (a.dt_softplus) d[i] = softplus2(d[i]);
+          if (a.dt_softplus) d[i] = softplus2<T>(d[i]);
           v[i] = mul2(d[i], x[1].pair(i));
         }
       }
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
             if (a.D) y[i] = fma2(Dv[i], x[0].pair(i), y[i]);
             if (a.z) {
               const F2 zi = z[0].pair(i);
-              y[i] = mul2(y[i], mul2(zi, sigmoid2(zi)));
+              y[i] = mul2(y[i], mul2(zi, sigmoid2<T>(zi)));
             }
             out.set_pair(i, y[i]);
           }
@@ -749,12 +749,12 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
 #pragma unroll
           for (int i = 0; i < me.kPairs; ++i) {
             d[i] = add2(dt.pair(i), bias[i]);
-            if (a.dt_softplus) d[i] = softplus2(d[i]);
+            if (a.dt_softplus) d[i] = softplus2<T>(d[i]);
             v[i] = mul2(d[i], x.pair(i));
             w[i] = dy.pair(i);
             if (a.z) {
               const F2 zi = z.pair(i);
-              w[i] = mul2(w[i], mul2(zi, sigmoid2(zi)));
+              w[i] = mul2(w[i], mul2(zi, sigmoid2<T>(zi)));
             }
           }
         }
@@ -783,13 +783,13 @@ __global__ void __launch_bounds__(BackwardTeam::kBlock, 2)
               const F2 xv = x.pair(i), dyv = dy.pair(i);
               F2 w = dyv;
               if (a.z) {
-                const F2 zv = z.pair(i), s = sigmoid2(zv);
+                const F2 zv = z.pair(i), s = sigmoid2<T>(zv);
                 w = mul2(w, mul2(zv, s));
                 const F2 yv = a.D ? fma2(Dv[i], xv, y[i]) : y[i];
                 oz.set_pair(i, mul2(mul2(dyv, yv), silu_grad2(zv, s)));
               }
               F2 gd = fma2(gB[i], xv, mul2(gA[i], same2(kLn2)));
-              if (a.dt_softplus) gd = mul2(gd, sigmoid2(add2(dt.pair(i), bias[i])));
+              if (a.dt_softplus) gd = mul2(gd, sigmoid2<T>(add2(dt.pair(i), bias[i])));
               F2 gx = mul2(gB[i], d[i]);
               if (a.D) gx = fma2(Dv[i], w, gx);
               ox.set_pair(i, gx);
@@ -1091,7 +1091,7 @@ __global__ void __launch_bounds__(128) seq_scan_step_kernel(pt_scan_args a, int 
     x = to_f<T>(static_cast<const T*>(a.x)[b * a.x_batch + c]);
     if (a.z) z = to_f<T>(static_cast<const T*>(a.z)[b * a.z_batch + c]);
     if (a.D) D = __ldg(a.D + c);
-    if (a.dt_softplus) delta = softplusf(delta);
+    if (a.dt_softplus) delta = softplusf<T>(delta);
     v = delta * x;
   }
   if (a.slots && named_before(a.slots, b, slot, tid, threads)) {
@@ -1157,7 +1157,7 @@ __global__ void __launch_bounds__(128) seq_scan_step_kernel(pt_scan_args a, int 
   if (own) {
     if (slot >= 0) {
       if (a.D) sum = fmaf(D, x, sum);
-      if (a.z) sum *= siluf(z);
+      if (a.z) sum *= siluf<T>(z);
     } else {
       sum = 0.f;
     }
