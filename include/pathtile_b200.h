@@ -425,7 +425,7 @@ typedef struct pt_scan_args {
 PT_API size_t pt_scan_checkpoint_bytes(const pt_scan_args* args);  /* of the sizes alone */
 PT_API size_t pt_scan_workspace_bytes(const pt_scan_args* args);
 PT_API int pt_scan(const pt_scan_args* args, void* ws, size_t ws_bytes, void* stream);
-PT_API size_t pt_scan_bwd_workspace_bytes(const pt_scan_args* args);
+PT_API size_t pt_scan_bwd_workspace_bytes(const pt_scan_args* args);  /* less where neither dB nor dC is wanted */
 PT_API int pt_scan_bwd(const pt_scan_args* args, void* ws, size_t ws_bytes, void* stream);
 PT_API int pt_scan_step(const pt_scan_args* args, void* stream);
 

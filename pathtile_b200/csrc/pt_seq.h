@@ -41,6 +41,8 @@ struct ScanPlan {
   int row_chunks;  // backward only: blocks along the batch, each looping over rows
 };
 ScanPlan scan_plan(const pt_scan_args& a, int sm_count, bool backward);
+// Floats of the partial sums of dB and dC in the backward workspace, behind the segments'.
+size_t bc_floats(const pt_scan_args& a, const ScanPlan& p);
 
 cudaError_t launch_norm_fwd(const pt_norm_args& a, int sm_count, cudaStream_t stream);
 cudaError_t launch_norm_bwd(const pt_norm_args& a, float* ws, int sm_count, cudaStream_t stream);

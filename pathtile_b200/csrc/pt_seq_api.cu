@@ -101,8 +101,14 @@ size_t scan_fwd_workspace(const pt_scan_args& a, int sm_count) { return segment_
 size_t scan_bwd_workspace(const pt_scan_args& a, int sm_count) {
   const ScanPlan p = scan_plan(a, sm_count, true);
   const size_t pieces = static_cast<size_t>(p.row_chunks) * p.segs;
-  const size_t rows = static_cast<size_t>(a.batch) * a.len * a.groups;
-  return segment_bytes(a, p) + sizeof(float) * (p.cblocks * rows * 8 * p.slices + pieces * a.dim * a.state + pieces * 2 * a.dim);
+  return segment_bytes(a, p) + sizeof(float) * (bc_floats(a, p) + pieces * a.dim * a.state + pieces * 2 * a.dim);
+}
+
+// Partial sums of dB and dC: one of all (padded) states for every step and block of channels, so 2 bytes per step and
+// channel up to 16 states, 8 up to 32 and 32 up to 64.
+size_t bc_floats(const pt_scan_args& a, const ScanPlan& p) {
+  if (!a.dB && !a.dC) return 0;
+  return static_cast<size_t>(p.cblocks) * a.batch * a.len * a.groups * 8 * p.slices;
 }
 
 }  // namespace seq

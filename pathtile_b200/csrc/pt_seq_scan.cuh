@@ -1251,7 +1251,7 @@ cudaError_t scan_bwd(const pt_scan_args& a, const ScanPlan& p, float* ws, cudaSt
     float* seg_h = ws;
     float* seg_d = ws + static_cast<size_t>(a.batch) * p.segs * a.dim * a.state;
     float* part_bc = ws + segment_floats(a, p);
-    float* part_p = part_bc + p.cblocks * rows * 8 * S;
+    float* part_p = part_bc + bc_floats(a, p);
     const long long blocks = static_cast<long long>(p.cblocks) * a.groups;
     if (blocks * a.batch * p.segs > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     cudaError_t e;
