@@ -432,6 +432,14 @@ __global__ void __launch_bounds__(ForwardTeam<T>::kBlock, 2)
       if (c < me.mine) seg_d[out * a.dim + me.c + c] = dsum[c];
 }
 
+// exp(delta A) h.  Of a whole segment the factor may be past the largest float where the product is not, so it
+// is applied as two square roots; a state of zero stays zero whatever the factor.
+__device__ __forceinline__ F2 carry(F2 delta, F2 A2, F2 h) {
+  const F2 root = ex2x2(mul2(fma2(delta, A2, same2(kCentre)), same2(0.5f)));
+  const F2 p = mul2(mul2(root, h), root);
+  return pack2(lo2(h) == 0.f ? 0.f : lo2(p), hi2(h) == 0.f ? 0.f : hi2(p));
+}
+
 // h <- exp(A sum delta of segment s) h + its own state.
 template <int S, class TEAM>
 __device__ __forceinline__ void join_segment(const pt_scan_args& a, const ScanDims& dm, const float* seg_h,
@@ -444,7 +452,7 @@ __device__ __forceinline__ void join_segment(const pt_scan_args& a, const ScanDi
   for (int i = 0; i < 2; ++i) {
     const float d = i < me.mine ? seg_d[row * a.dim + me.c + i] : 0.f;
 #pragma unroll
-    for (int p = 0; p < 2; ++p) h[i][p] = fma2(decay(pack2(d, d), A2[i][p]), h[i][p], l[i][p]);
+    for (int p = 0; p < 2; ++p) h[i][p] = add2(carry(pack2(d, d), A2[i][p], h[i][p]), l[i][p]);
   }
 }
 

@@ -100,6 +100,7 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Te
     states]`` where each group serves channels / groups neighbouring channels,
     in x's type.  ``initial_state`` is ``[batch, channels, states]`` float32
     (zeros without it); with ``return_final_state`` the result is ``(y, state)``.
+    A step's ``exp(delta A)`` is a float32: states may grow, by up to e^88 a step.
     Differentiable in all tensors but lengths, through y and the final state.
     """
     out = (_native or _load()).selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state,
