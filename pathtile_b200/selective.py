@@ -89,26 +89,28 @@ class SelectiveBlock(nn.Module):
         """Branch output and residual stream for ``x[batch, length, hidden]``.
 
         ``cache`` (one row per batch row) holds what came before and is brought
-        up to each row's end: in place, or, while gradients are recorded, with
-        new tensors (no gradient passes through it); ``lengths`` as in
-        :func:`selective_scan`.
+        up to each row's end, in place, so that captured steps read it; no
+        gradient passes through it.  ``lengths`` as in :func:`selective_scan`.
         """
         h, residual = self._enter(x, residual)
         u, z = self.in_proj(h).chunk(2, dim=-1)
         keep = cache is not None
-        u = causal_conv(u, self.conv_weight, self.conv_bias, silu=True, initial_state=cache.window if keep else None,
+        window = state = None
+        if keep:
+            window, state = cache.window, cache.state
+            if torch.is_grad_enabled():  # what the backward pass saves must stay, and the cache moves on
+                window, state = window.detach().clone(), state.detach().clone()
+        u = causal_conv(u, self.conv_weight, self.conv_bias, silu=True, initial_state=window,
                         return_final_state=keep, lengths=lengths)
         if keep:
             u, window = u
         dt, B, C = self._operands(u)
         A, D, dt_bias = self._scan_params()
         y = selective_scan(u, dt, A, B, C, D, None, dt_bias, dt_softplus=True,
-                           initial_state=cache.state if keep else None, return_final_state=keep, lengths=lengths)
+                           initial_state=state, return_final_state=keep, lengths=lengths)
         if keep:
             y, state = y
-            if torch.is_grad_enabled():  # what the backward pass has saved must stay: the cache gets new tensors
-                cache.window, cache.state = window.detach(), state.detach()
-            else:
+            with torch.no_grad():
                 cache.window.copy_(window)
                 cache.state.copy_(state)
         return self._leave(y, z), residual
