@@ -72,9 +72,9 @@ ScanPlan scan_plan(const pt_scan_args& a, int sm_count, bool backward) {
   p.cblocks = static_cast<int>(cdiv(a.dim / a.groups, p.ch));
   const long long blocks = static_cast<long long>(p.cblocks) * a.groups * a.batch;
   // Two blocks fill an SM.  A segment costs its exponentials twice, so the length is cut only where whole rows leave
-  // more than 40 % of those places empty; at least 64 steps keep the join of the states before it short.
-  long long segs = 1;
-  if (blocks > 0 && 10 * blocks < 12LL * sm_count) segs = 2LL * sm_count / blocks;
+  // half of those places empty or more (as many segments as fill them); at least 64 steps keep the join of the states
+  // before it short.
+  long long segs = blocks > 0 ? 2LL * sm_count / blocks : 1;
   const long long most = cdiv(a.len, 64);
   segs = segs < most ? segs : most;
   segs = segs > 1 ? segs : 1;
