@@ -292,6 +292,10 @@ __device__ __forceinline__ void get_pairs(const float* src, F2 (&v)[(E + 1) / 2]
 constexpr unsigned kSlotPastCache = 1u << 7, kSlotTwice = 1u << 8;
 
 // Whether a row before `row` names the slot as well.  Every thread of the block calls it.
+// Every block of a row reads the slots of all rows before it, which grows with the square
+// of the batch.  Steps of 2048 channels (16 states, 4 taps, bf16) without and with slots:
+// 256 rows, scan 20.1 and 22.5 us, convolution 8.2 and 10.2; 4096 rows, 188 and 274, 35 and
+// 53; 16384 rows, 723 and 1966, 117 and 295.
 __device__ __forceinline__ bool named_before(const int* __restrict__ slots, int row, int slot, int thread, int threads) {
   int twice = 0;
   if (slot >= 0)

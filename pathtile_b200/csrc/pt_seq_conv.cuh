@@ -6,8 +6,9 @@
 // memory (plus K-1 steps of overlap per stretch).  All rows' steps are laid end
 // to end and cut into equal stretches, so that every thread has the same work
 // whatever the batch; a stretch that crosses into the next row starts anew
-// there.  V is the widest word (up to 16 bytes forward, 8 backward) that every
-// pointer, stride and row length allows.  The loads of the next U steps are
+// there.  V is a word of 16 bytes forward and 8 backward where every pointer,
+// stride and row length allows it (and there are up to four taps), else two
+// elements, else one.  The loads of the next U steps are
 // under way while U steps are computed, in packed fp32 arithmetic.  The taps
 // come through shared memory: read straight, a warp's taps lie V x K floats
 // apart and cost more than the steps.
@@ -457,10 +458,10 @@ template <int VMAX, class F>
 cudaError_t by_width_taps(int v, int k, F&& fn) {
   auto taps = [&](auto vc) -> cudaError_t {
     switch (k) {
-            case 1: return fn(vc, std::integral_constant<int, 1>());
+      case 1: return fn(vc, std::integral_constant<int, 1>());
       case 2: return fn(vc, std::integral_constant<int, 2>());
       case 3: return fn(vc, std::integral_constant<int, 3>());
-            case 4: return fn(vc, std::integral_constant<int, 4>());
+      case 4: return fn(vc, std::integral_constant<int, 4>());
       default: break;
     }
     if constexpr (decltype(vc)::value <= 2) {

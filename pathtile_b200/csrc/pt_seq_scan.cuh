@@ -62,7 +62,7 @@ struct ScanTeam {
 // four are enough and leave the scanners more registers (762 us; with eight, which
 // spill, 827).
 // fp32 rows on their way take twice the registers (2048 x 48 x 256: 215 us, 283 us
-// with the other split).
+// with the other split; 8 more with the exponentials of fp32 calls).
 template <class T>
 using ForwardTeam = ScanTeam<256, sizeof(T) == 4 ? 80 : 112, sizeof(T) == 4 ? 80 : 64>;
 using BackwardTeam = ScanTeam<128, 136, 120>;
@@ -1040,7 +1040,7 @@ __global__ void seq_scan_bc_kernel(const float* part, int cblocks, long long row
 // what the others need of it crosses by shuffles, so nothing is computed twice.
 // Bound by reading and writing the states: those, and all else, are on their way
 // while the block looks whether an earlier row has the slot.  256 rows of 4096
-// channels with 16 states: 31 us (4.3 TB/s; 53 us with every lane computing its
+// channels with 16 states: 31 us (4.6 TB/s; 53 us with every lane computing its
 // channel's delta and gate itself); one row of 2048: 2.6 us.
 template <int S>
 constexpr int kStepChannels = S == 2 ? 2 : 4;

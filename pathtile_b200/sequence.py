@@ -79,7 +79,9 @@ def causal_conv_step(state: Tensor, x: Tensor, weight: Tensor, bias: Tensor | No
     window b without ``slots``.  A negative slot marks a padding row: its output
     is 0 and no window is touched.  So is a row whose slot is past the cache, or
     was named by an earlier row of the batch; bits 7 and 8 of
-    :func:`pathtile_b200.ops.device_error` report that.
+    :func:`pathtile_b200.ops.device_error` report that.  (Each row looks through
+    the slots of all rows before it: a tenth of a step's time at 256 rows, more
+    than the step itself at some ten thousand.)
     """
     return (_native or _load()).causal_conv_step(state, x, weight, bias, silu, slots)
 
@@ -101,6 +103,9 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Te
     in x's type.  ``initial_state`` is ``[batch, channels, states]`` float32
     (zeros without it); with ``return_final_state`` the result is ``(y, state)``.
     A step's ``exp(delta A)`` is a float32: states may grow, by up to e^88 a step.
+    For its backward pass a call keeps a quarter of a byte per step, channel and
+    state; for the gradients of B and C that pass takes 2 bytes of scratch per step
+    and channel with up to 16 states, 8 with up to 32, 32 with more.
     Differentiable in all tensors but lengths, through y and the final state.
     """
     out = (_native or _load()).selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state,
