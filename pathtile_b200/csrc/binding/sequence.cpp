@@ -215,7 +215,7 @@ struct Backward<OP, variable_list(A...)> {
       BelowAutograd below;
       out = call(args...);
     }
-    once(out);
+    if (wants_grad({tensor_of(args)...})) once(out);
     return out;
   }
   static Tensor tensor_of(const Tensor& t) { return t; }

@@ -9,10 +9,14 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
 import pathtile_b200 as pt
-
-pytestmark = pytest.mark.usefixtures("native_lib")
+from pathtile_b200 import sequence
 
 B, L, D, N, K = 2, 37, 24, 8, 4
+
+
+@pytest.fixture(autouse=True)
+def operators(native_lib):
+    sequence._load()
 
 
 def f(*shape, dtype=torch.float32, device="meta"):
@@ -159,6 +163,16 @@ def test_transforms_without_a_rule_say_so():
             torch.func.grad(lambda x: one(x).sum())(v["x"])
         with pytest.raises((RuntimeError, ValueError)):
             torch.func.jvp(one, (v["x"],), (v["x"],))
+
+
+def test_a_backward_operator_called_by_name_asks_for_no_gradient_of_its_own_accord():
+    """As a traced gradient calls it: with plain tensors its results are plain too."""
+    v = conv_inputs()
+    args = [f(B, L, D), None, v["x"], v["weight"], None, None, None, True, [True, True, False, False]]
+    assert not any(t.requires_grad for t in torch.ops.pathtile_b200.causal_conv_backward(*args))
+    args[3] = args[3].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.ops.pathtile_b200.causal_conv_backward(*args)[0].sum().backward()
 
 
 def test_operators_called_by_name_check_their_arguments():
